@@ -377,6 +377,135 @@ MLXCAT_API int mlxcat_op_dequant_q4(const uint32_t *wq, const uint16_t *scales, 
 MLXCAT_API int mlxcat_op_gemm_f16(const uint16_t *w, int32_t N, int32_t K, const uint16_t *x, int32_t M,
                                   int32_t epilogue, void *out, int32_t ldo, int32_t *err_flag, void *stream);
 
+/* ---- paged KV cache ------------------------------------------------------------
+ * Operators for a host that keeps its keys and values in blocks (the reference's
+ * prefix cache chains 256-token blocks, TrackA/BlockAwarePrefixCache.swift:57-87)
+ * instead of one contiguous slot per row: append with normalisation and rotary
+ * positions, attention of single tokens and verify groups, the same for a batch
+ * whose first blocks are shared, and the causal attention of several prompts at
+ * once.  All take device pointers and a stream of the current device, use no
+ * memory but their arguments' (each call its own workspace: calls whose kernels
+ * may overlap must not share one), read no device value on the host and can be
+ * captured in a graph.
+ *
+ * Element types: the cache, queries and outputs are fp16 or bf16 (one type per
+ * call); rope_append also reads fp32 (a projection's accumulator). */
+#define MLXCAT_F16 0
+#define MLXCAT_BF16 1
+#define MLXCAT_F32 2
+
+/* The cache: element (page, head, token, d) of k and v sits at page *
+ * page_stride + head * head_stride + token * token_stride + d (strides in
+ * elements, multiples of 8, elements must not overlap; k and v 16-byte
+ * aligned), so [page][head][token][d], [page][token][head][d] and slices of
+ * larger buffers are all described.  page_size is a power of two, 8..65536;
+ * head_dim 64 or 128.  Key p of row r is token p % page_size of page
+ * page_table[r * max_pages + p / page_size] (device int32). */
+typedef struct {
+    void *k, *v;
+    const int32_t *page_table;
+    int64_t page_stride, head_stride, token_stride;
+    int32_t dtype;                /* MLXCAT_F16 / MLXCAT_BF16               */
+    int32_t n_pages, page_size, n_kv_heads, head_dim;
+    int32_t rows, max_pages;      /* shape of page_table                    */
+} mlxcat_paged_kv;
+
+/* Rotary positions (the RoPE of the model's attention blocks, mlx-swift-lm,
+ * un-vendored).  mlxcat_rope_init (host only) fills the plan: pair i of the
+ * first rotary_dim features (even, 2..256) turns by pos * f_i, f_i =
+ * theta^(-2i / rotary_dim) changed by the scaling; pairs are (i, i +
+ * rotary_dim / 2) for MLXCAT_ROPE_HALF and (2i, 2i + 1) for
+ * MLXCAT_ROPE_INTERLEAVED.  scaling NULL or kind NONE: as is.
+ *   LINEAR: f / factor.
+ *   LLAMA3: by the turns n = original_max_position * f / 2 pi of a pair within
+ *     the original context: f / factor below low_freq_factor turns, f above
+ *     high_freq_factor, linear in n between.
+ *   YARN: f / factor for pairs that turn less than beta_slow times, f for those
+ *     that turn more than beta_fast times, linear in the pair's index between;
+ *     cos and sin times mscale (0: 0.1 ln(factor) + 1). */
+#define MLXCAT_ROPE_HALF 0
+#define MLXCAT_ROPE_INTERLEAVED 1
+#define MLXCAT_ROPE_SCALE_NONE 0
+#define MLXCAT_ROPE_SCALE_LINEAR 1
+#define MLXCAT_ROPE_SCALE_LLAMA3 2
+#define MLXCAT_ROPE_SCALE_YARN 3
+typedef struct {
+    int32_t kind, original_max_position;
+    double factor, low_freq_factor, high_freq_factor, beta_fast, beta_slow, mscale;
+} mlxcat_rope_scaling;
+typedef struct {
+    int32_t rotary_dim, layout;
+    float mscale;
+    int32_t reserved;
+    double turns[128];            /* f_i / 2 pi                             */
+} mlxcat_rope;
+MLXCAT_API int mlxcat_rope_init(mlxcat_rope *rope, int32_t rotary_dim, int32_t layout, double theta,
+                                const mlxcat_rope_scaling *scaling);
+
+/* Per-head RMSNorm (q_norm, k_norm: fp32 [head_dim], each may be NULL), rotary
+ * positions (rope may be NULL) and append, for M tokens of row trow[m] at
+ * position tpos[m] (device int32): q [n_heads], k and v [n_kv_heads] heads of
+ * head_dim per token, in_dtype, tokens *_stride elements apart (multiples of 8,
+ * 16-byte aligned; the three parts of a fused projection are such slices).
+ * q_out [M][n_heads][head_dim] in the cache's type, not overlapping the inputs;
+ * q and q_out may both be NULL (append only).  A token with trow < 0 is padding:
+ * nothing is written for it.  A row, position or page outside the table or the
+ * cache sets *err (device int, may be NULL) and its key and value are not
+ * written.  Two tokens with the same row and position leave one of the two. */
+MLXCAT_API int mlxcat_op_rope_append(const mlxcat_paged_kv *kv, const mlxcat_rope *rope, const void *q,
+                                     const void *k, const void *v, int32_t in_dtype, int64_t q_stride,
+                                     int64_t k_stride, int64_t v_stride, int32_t M, int32_t n_heads,
+                                     const float *q_norm, const float *k_norm, float eps,
+                                     const int32_t *trow, const int32_t *tpos, void *q_out, int32_t *err,
+                                     void *stream);
+
+/* mlxcat_op_attention on the paged cache: token m of row trow[m] sees keys
+ * 0..tpos[m]; tokens come in groups of qg, all of one row (qg = 1: single
+ * tokens, k + 1: a verify step; a group may end in padding tokens, trow < 0).
+ * q, out [M][n_heads][head_dim] in the cache's type; scale 0: 1 / sqrt(head_dim).
+ * A token that sees no key (tpos < 0) gets zeros, a padding token's output is
+ * left as it was.  A row or position outside the table sets *err (device int,
+ * may be NULL) and is cut to the table; a page id outside the cache sets it and
+ * reads as zeros.  Keys past a group's last position are not read; a NaN or
+ * infinite V entry reaches every token of a group that may see it. */
+MLXCAT_API size_t mlxcat_op_paged_attention_workspace(int32_t M, int32_t qg, int32_t n_heads, int32_t n_kv_heads,
+                                                      int32_t head_dim);
+MLXCAT_API int mlxcat_op_paged_attention(const mlxcat_paged_kv *kv, const void *q, int32_t M, int32_t qg,
+                                         int32_t n_heads, float scale, const int32_t *trow,
+                                         const int32_t *tpos, void *out, void *workspace,
+                                         size_t workspace_bytes, int32_t *err, void *stream);
+
+/* The same result for a batch whose rows share their first prefix_len keys
+ * (a multiple of page_size; page_table[r] starts with the same prefix_len /
+ * page_size pages for every row r of the batch): those pages are read once for
+ * all tokens, on the tensor cores.  prefix_len 0 is mlxcat_op_paged_attention. */
+MLXCAT_API size_t mlxcat_op_shared_prefix_attention_workspace(int32_t M, int32_t qg, int32_t n_heads,
+                                                              int32_t n_kv_heads, int32_t head_dim,
+                                                              int32_t prefix_len);
+MLXCAT_API int mlxcat_op_shared_prefix_attention(const mlxcat_paged_kv *kv, int32_t prefix_len, const void *q,
+                                                 int32_t M, int32_t qg, int32_t n_heads, float scale,
+                                                 const int32_t *trow, const int32_t *tpos, void *out,
+                                                 void *workspace, size_t workspace_bytes, int32_t *err,
+                                                 void *stream);
+
+/* mlxcat_op_prefill_attention for several prompts laid end to end: sequence s
+ * owns queries cu_q[s]..cu_q[s+1]-1 of q [Tq][n_heads][head_dim] and keys
+ * cu_k[s]..cu_k[s+1]-1 of k, v [Tk][n_kv_heads][head_dim] (tokens *_stride
+ * elements apart, multiples of 8, 16-byte aligned; cu_q, cu_k device int32
+ * [n_seq + 1], not decreasing).  causal: query i of a sequence of nq queries and
+ * nk keys sees keys 0..nk - nq + i (the queries are its last tokens), else all
+ * nk.  A query that sees no key gets zeros; tokens outside the sequences are
+ * left as they were.  out [Tq][n_heads][head_dim].  No sequence's values reach
+ * another's; within a causal sequence a NaN or infinite V entry can reach
+ * queries up to 127 positions before it.  n_heads / n_kv_heads <= 64.  *err
+ * (device int, may be NULL) becomes non-zero if a pipeline wait timed out. */
+MLXCAT_API int mlxcat_op_packed_attention(const void *q, const void *k, const void *v, int32_t dtype,
+                                          int64_t q_stride, int64_t k_stride, int64_t v_stride, int32_t Tq,
+                                          int32_t Tk, const int32_t *cu_q, const int32_t *cu_k, int32_t n_seq,
+                                          int32_t causal, int32_t n_heads, int32_t n_kv_heads,
+                                          int32_t head_dim, float scale, void *out, int32_t *err,
+                                          void *stream);
+
 /* Seeded N(0, stddev) weights quantised to MLX affine q4 g64 (bit-identical
  * with the CPU restatement). */
 MLXCAT_API int mlxcat_op_synth_q4(uint64_t seed, uint32_t tensor_id, float stddev, int32_t N, int32_t K,

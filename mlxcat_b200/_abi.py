@@ -74,8 +74,38 @@ class RowsC(C.Structure):
     ]
 
 
+F16, BF16, F32 = 0, 1, 2
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_LLAMA3, ROPE_SCALE_YARN = 0, 1, 2, 3
+
+
+class PagedKVC(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p),
+        ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64),
+        ("dtype", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+        ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rows", C.c_int32), ("max_pages", C.c_int32),
+    ]
+
+
+class RopeScalingC(C.Structure):
+    _fields_ = [
+        ("kind", C.c_int32), ("original_max_position", C.c_int32), ("factor", C.c_double),
+        ("low_freq_factor", C.c_double), ("high_freq_factor", C.c_double), ("beta_fast", C.c_double),
+        ("beta_slow", C.c_double), ("mscale", C.c_double),
+    ]
+
+
+class RopeC(C.Structure):
+    _fields_ = [
+        ("rotary_dim", C.c_int32), ("layout", C.c_int32), ("mscale", C.c_float), ("reserved", C.c_int32),
+        ("turns", C.c_double * 128),
+    ]
+
+
 # name -> (restype, argtypes)
 _vp, _i32, _u32, _u64, _f32, _sz = C.c_void_p, C.c_int32, C.c_uint32, C.c_uint64, C.c_float, C.c_size_t
+_i64, _f64, _kvp = C.c_int64, C.c_double, C.POINTER(PagedKVC)
 _vp3 = C.c_void_p * 3   # const T *const [3]: gate, up, down
 PROTOTYPES = {
     "mlxcat_ctx_create": (C.c_int, [C.POINTER(ModelConfigC), _i32, C.POINTER(_vp)]),
@@ -137,6 +167,16 @@ PROTOTYPES = {
     "mlxcat_op_moe_workspace": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "mlxcat_op_moe": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp3, _vp3, _vp3,
                                 _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mlxcat_rope_init": (C.c_int, [C.POINTER(RopeC), _i32, _i32, _f64, C.POINTER(RopeScalingC)]),
+    "mlxcat_op_rope_append": (C.c_int, [_kvp, C.POINTER(RopeC), _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _i32,
+                                        _vp, _vp, _f32, _vp, _vp, _vp, _vp, _vp]),
+    "mlxcat_op_paged_attention_workspace": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "mlxcat_op_paged_attention": (C.c_int, [_kvp, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "mlxcat_op_shared_prefix_attention_workspace": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "mlxcat_op_shared_prefix_attention": (C.c_int, [_kvp, _i32, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp,
+                                                    _sz, _vp, _vp]),
+    "mlxcat_op_packed_attention": (C.c_int, [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _i32, _i32,
+                                             _i32, _i32, _i32, _f32, _vp, _vp, _vp]),
     "mlxcat_op_draft": (C.c_int, [C.POINTER(RowsC), C.POINTER(SpecConfigC), _vp, _vp, _vp, _vp, _vp]),
     "mlxcat_op_accept_workspace": (_sz, [_i32, _i32]),
     "mlxcat_op_accept": (C.c_int, [C.POINTER(RowsC), C.POINTER(SpecConfigC), _vp, _vp, _vp, _i32,

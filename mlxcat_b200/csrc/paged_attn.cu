@@ -1,0 +1,621 @@
+// paged_attn.cu -- attention of single tokens and verify groups over a paged
+// cache:  out[m, h] = sum_p softmax_p(scale q[m,h].k_p) v_p,  p <= tpos[m].
+//
+// Bound by HBM: every K and V byte of a row is read once and meets only the
+// qg * G query rows of its KV head, far below the ridge.  So the kernel is a
+// stream with as little between the loads as possible:
+//
+// * A warp owns 16 keys at a time and its own ring of cp.async stages (no CTA
+//   barrier in the loop).  Pages are looked up 32 tiles at a time, a lane each.
+// * The products are transposed: S^T = K Q^T with the 16 keys as the M of
+//   mma.m16n8k16 and 8 query rows as its N, then O^T = V^T P^T.  A group of 4
+//   or 8 query rows fills the N = 8 tile (as M it would pad to 16), and the
+//   accumulator of S^T, packed to 16 bits and turned by movmatrix, is the B
+//   operand of the second product.  The row sums come from the same packed P,
+//   by one more product with a matrix of ones, so numerator and denominator
+//   round alike.
+// * P = 2^(z - m), z in log2 units; the reference m moves only when a score is
+//   more than 8 above it (P <= 256 fits fp16), so most tiles have no
+//   cross-lane maximum and no rescaling.
+// * Rows differ in length and only the device knows it: the units (64 keys) of
+//   all (group, KV head, query tile) items are laid end to end and every CTA
+//   takes an equal stretch.  An item inside one CTA is finished there; the
+//   others leave (O, max, sum) partials, which attn_join merges in order, so
+//   results do not depend on timing.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "paged.h"
+#include "tc.cuh"
+
+namespace mlxcat {
+
+namespace {
+
+constexpr int PW = 4;              // warps per CTA
+constexpr int PT = PW * 32;
+constexpr int TK = 16;             // keys per warp tile
+constexpr int UNIT = PW * TK;      // keys per unit
+constexpr int ST = 3;              // ring stages per warp
+constexpr int CTAS_PER_SM = 2;
+
+template <typename T>
+struct Half2;
+template <>
+struct Half2<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static constexpr uint32_t ones = 0x3C003C00u;
+    static __device__ __forceinline__ void mma(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <>
+struct Half2<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static constexpr uint32_t ones = 0x3F803F80u;
+    static __device__ __forceinline__ void mma(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+__device__ __forceinline__ void ldm4(uint32_t *d, uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t *d, uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void cpa16(uint32_t s, const void *g, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(g), "r"(bytes) : "memory");
+}
+
+// What a group of tokens sees: its row and one past its last key (clamped to
+// what the table holds).  Every lane of the warp gets the same answer.
+struct Group {
+    int row, kend;
+};
+__device__ __forceinline__ Group group_of(const PagedKV &kv, const PagedQuery &a, int grp) {
+    const int lane = threadIdx.x & 31, t0 = grp * a.qg, n = min(a.qg, a.M - t0);
+    int row = -1, kend = 0;
+    for (int j = lane; j < n; j += 32) {
+        const int r = __ldg(a.trow + t0 + j), p = __ldg(a.tpos + t0 + j);
+        if (r >= 0) {
+            row = max(row, r);
+            kend = max(kend, p == 0x7fffffff ? p : p + 1);
+        }
+    }
+    row = __reduce_max_sync(0xffffffffu, row);
+    kend = __reduce_max_sync(0xffffffffu, kend);
+    const int cap = paged_capacity(kv);
+    if (row >= kv.rows || kend > cap) {
+        if (lane == 0 && a.err) atomicExch(a.err, row >= kv.rows ? PE_ROW : PE_POS);
+        kend = row >= kv.rows ? 0 : cap;
+    }
+    return {row, kend};
+}
+// the same for one thread (the scan over groups)
+__device__ __forceinline__ int group_units(const PagedKV &kv, const PagedQuery &a, int grp, int key_begin) {
+    const int t0 = grp * a.qg, n = min(a.qg, a.M - t0);
+    int row = -1, kend = 0;
+    for (int j = 0; j < n; ++j) {
+        const int r = __ldg(a.trow + t0 + j), p = __ldg(a.tpos + t0 + j);
+        if (r >= 0) {
+            row = max(row, r);
+            kend = max(kend, p == 0x7fffffff ? p : p + 1);
+        }
+    }
+    if (row < 0 || row >= kv.rows) return 0;
+    kend = min(kend, paged_capacity(kv));
+    return kend > key_begin ? (int)(((int64_t)kend - key_begin + UNIT - 1) / UNIT) : 0;
+}
+
+__device__ __forceinline__ int64_t cta_begin(int c, int64_t U, int C) { return (int64_t)c * U / C; }
+
+// What a partial with maximum m and sum l weighs against the maximum mx of all.
+// A partial that saw nothing (m = -inf, l = 0) weighs nothing; one whose scores
+// were all NaN keeps its NaN sum.
+__device__ __forceinline__ float weight_of(float m, float l, float mx) {
+    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : tc::ex2_approx(m - mx);
+}
+
+// One float4 more per row keeps the merge's shared-memory stores apart.
+template <int D, int NT>
+struct PagedShape {
+    static constexpr int STAGE = 2 * TK * D * 2;            // K and V of one tile, bytes
+    static constexpr int RING = PW * ST * STAGE;
+    static constexpr int QR = NT * 8;                       // query rows of an item
+    static constexpr int OP = D + 4;
+    static constexpr int MERGE = PW * QR * (OP + 2) * 4;
+    static constexpr int SMEM = RING > MERGE ? RING : MERGE;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(PT, CTAS_PER_SM)
+paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force_partial, float *__restrict__ o_part,
+                  float *__restrict__ ml_part, int2 *__restrict__ meta) {
+    using S = PagedShape<D, NT>;
+    constexpr int CH = D / 8;            // 16-byte chunks per key
+    constexpr int RPI = 32 / CH;         // keys per load instruction of a warp
+    extern __shared__ __align__(128) unsigned char psm[];
+    __shared__ int64_t wsum[PW];
+    __shared__ int64_t start_s[2];       // group of the first unit, units before it
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    const int Hq = a.n_heads, Hkv = kv.n_kv, G = Hq / Hkv;
+    const int groups = (a.M + a.qg - 1) / a.qg;
+    const int qts = (a.qg * G + S::QR - 1) / S::QR;
+    const int per_group = Hkv * qts;     // items of a group: (query tile, KV head)
+
+    griddep_launch_dependents();
+    griddep_wait();
+
+    // ---- where this CTA's stretch of units starts: thread x sums the groups of
+    // its chunk, a scan gives the total and the chunk that holds the start
+    const int per = (groups + PT - 1) / PT;
+    int64_t mine = 0;
+    {
+        const int g0 = threadIdx.x * per, g1 = min(groups, g0 + per);
+        for (int i = g0; i < g1; ++i) mine += group_units(kv, a, i, key_begin);
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    int64_t before = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < PW; ++w) {
+        if (w < warp) before += wsum[w];
+        total += wsum[w];
+    }
+    const int64_t U = total * per_group;
+    const int C = (int)min((int64_t)gridDim.x, U);   // CTAs that work
+    const int64_t u0 = blockIdx.x < C ? cta_begin(blockIdx.x, U, C) : 0;
+    const int64_t u1 = blockIdx.x < C ? cta_begin(blockIdx.x + 1, U, C) : 0;
+    if (u1 > u0 && before * per_group <= u0 && u0 < (before + mine) * per_group) {
+        int64_t acc = before * per_group;
+        int i = threadIdx.x * per;
+        for (;; ++i) {
+            const int64_t n = (int64_t)group_units(kv, a, i, key_begin) * per_group;
+            if (u0 < acc + n) break;
+            acc += n;
+        }
+        start_s[0] = i;
+        start_s[1] = acc;
+    }
+    __syncthreads();
+
+    // ---- groups without keys here: nothing else writes their outputs
+    for (int i = blockIdx.x; i < groups; i += gridDim.x) {
+        if (warp != 0) continue;
+        if (group_of(kv, a, i).kend > key_begin) continue;
+        for (int x = lane; x < per_group; x += 32) meta[(size_t)i * per_group + x] = make_int2(0, -1);
+        if (force_partial) continue;
+        const int t0 = i * a.qg, n = min(a.qg, a.M - t0);
+        for (int j = 0; j < n; ++j) {
+            if (__ldg(a.trow + t0 + j) < 0) continue;   // padding stays as it was
+            uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + (size_t)(t0 + j) * Hq * D);
+            for (int x = lane; x < Hq * D / 8; x += 32) dst[x] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    if (u1 <= u0) return;
+
+    int grp = (int)start_s[0];
+    int64_t ubase = start_s[1];          // units before this group
+    Group gi = group_of(kv, a, grp);
+    int gu = gi.kend > key_begin ? (gi.kend - key_begin + UNIT - 1) / UNIT : 0;   // units per item
+    unsigned char *ring = psm + warp * (ST * S::STAGE);
+    const uint32_t ring_a = tc::smem_u32(ring);
+    const int ch = lane % CH, r0 = lane / CH;
+
+    for (int64_t u = u0; u < u1;) {
+        while (u >= ubase + (int64_t)gu * per_group) {
+            ubase += (int64_t)gu * per_group;
+            gi = group_of(kv, a, ++grp);
+            gu = gi.kend > key_begin ? (gi.kend - key_begin + UNIT - 1) / UNIT : 0;
+        }
+        const int x = (int)((u - ubase) / gu);                 // item of the group
+        const int64_t ib = ubase + (int64_t)x * gu;            // its first unit
+        const int ua = (int)(u - ib), ub = (int)min((int64_t)gu, u1 - ib);
+        const bool whole = ua == 0 && ub == gu;
+        const int h = x / qts, qt = x - h * qts;
+        const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
+        const int nq = min(S::QR, ntok * G - qt * S::QR);      // may be <= 0 in a last, short group
+        const size_t item = (size_t)grp * per_group + x;
+        u = ib + ub;
+
+        // ---- query rows as B operands, key limits per column
+        uint32_t qf[NT][D / 16][2];
+        int lim[NT][2];
+        int lim_min = 0x7fffffff;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + g;
+            const int rr = qt * S::QR + r;
+            const bool ok = r < nq;
+            const T *src = reinterpret_cast<const T *>(a.q) +
+                           ((size_t)(t0 + (ok ? rr / G : 0)) * Hq + h * G + (ok ? rr % G : 0)) * D;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+                qf[nt][ks][0] = ok ? __ldg(reinterpret_cast<const uint32_t *>(src + ks * 16 + 2 * t)) : 0u;
+                qf[nt][ks][1] = ok ? __ldg(reinterpret_cast<const uint32_t *>(src + ks * 16 + 8 + 2 * t)) : 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = nt * 8 + 2 * t + e, cc = qt * S::QR + c;
+                int l = 0x7fffffff;
+                if (c < nq && __ldg(a.trow + t0 + cc / G) >= 0) l = __ldg(a.tpos + t0 + cc / G);
+                lim[nt][e] = l;
+                lim_min = min(lim_min, l);
+            }
+        }
+        lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+
+        float o[D / 16][NT][4], ls[NT][4], mr[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            mr[nt][0] = mr[nt][1] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ls[nt][i] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[mt][nt][i] = 0.f;
+        }
+
+        const int steps = ub - ua;
+        const int kfirst = key_begin + ua * UNIT + warp * TK;   // key 0 of step 0 (fits: below the table's capacity + UNIT)
+        const T *kb = reinterpret_cast<const T *>(kv.k) + (int64_t)h * kv.head_stride;
+        const T *vb = reinterpret_cast<const T *>(kv.v) + (int64_t)h * kv.head_stride;
+        const int32_t *table = kv.table + (size_t)gi.row * kv.max_pages;
+        const int pmask = (1 << kv.page_shift) - 1;
+        int pid[2] = {-1, -1};       // lane l: pages of the two 8-key halves of step (32 batch + l)
+        auto lookup = [&](int step0) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int64_t key = (int64_t)kfirst + (int64_t)(step0 + lane) * UNIT + 8 * e;
+                int p = -1;
+                if (step0 + lane < steps && key < gi.kend) {
+                    p = __ldg(table + (key >> kv.page_shift));
+                    if (p < 0 || p >= kv.n_pages) {
+                        p = -1;
+                        if (a.err) atomicExch(a.err, PE_PAGE);
+                    }
+                }
+                pid[e] = p;
+            }
+        };
+        auto stage = [&](int s) {
+            if ((s & 31) == 0) lookup(s);
+            const int p0 = __shfl_sync(0xffffffffu, pid[0], s & 31), p1 = __shfl_sync(0xffffffffu, pid[1], s & 31);
+            const uint32_t dst = ring_a + (uint32_t)(s % ST) * S::STAGE;
+            const int key0 = kfirst + s * UNIT;
+#pragma unroll
+            for (int i = 0; i < TK / RPI; ++i) {
+                const int r = r0 + i * RPI, key = key0 + r;
+                const int p = r < 8 ? p0 : p1;
+                const bool ok = key < gi.kend && p >= 0;
+                const int64_t off = ok ? (int64_t)p * kv.page_stride + (int64_t)(key & pmask) * kv.token_stride + ch * 8 : 0;
+                const uint32_t so = dst + (uint32_t)(r * D * 2 + ((ch ^ (r & 7)) << 4));
+                cpa16(so, kb + off, ok ? 16 : 0);
+                cpa16(so + TK * D * 2, vb + off, ok ? 16 : 0);
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < ST - 1; ++s) {
+            if (s < steps) stage(s);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        }
+        for (int s = 0; s < steps; ++s) {
+            __syncwarp();            // every lane has read the stage that is filled now
+            if (s + ST - 1 < steps) stage(s + ST - 1);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 1) : "memory");
+            __syncwarp();
+            const int key0 = kfirst + s * UNIT;
+            if (key0 >= gi.kend) continue;   // no key of this tile (a last unit)
+            const uint32_t ka = ring_a + (uint32_t)(s % ST) * S::STAGE, va = ka + TK * D * 2;
+            float sc[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+            {
+                const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    uint32_t f[4];
+                    ldm4(f, ka + (uint32_t)(r * D * 2 + (((ks * 2 + (lane >> 4)) ^ (r & 7)) << 4)));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) Half2<T>::mma(sc[nt], f, qf[nt][ks][0], qf[nt][ks][1]);
+                }
+            }
+            if (key0 + TK - 1 > lim_min || key0 + TK > gi.kend) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = key0 + g + (i >> 1) * 8;
+                        if (key > lim[nt][i & 1] || key >= gi.kend) sc[nt][i] = -INFINITY;
+                    }
+            }
+            bool raise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[nt][i] *= a.scale_log2;
+                    raise |= sc[nt][i] > mr[nt][i & 1] + 8.f;
+                }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(sc[nt][e], sc[nt][2 + e]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float mn = fmaxf(mr[nt][e], mx);
+                        const float al = mr[nt][e] == -INFINITY ? 0.f : tc::ex2_approx(mr[nt][e] - mn);
+                        mr[nt][e] = mn;
+                        ls[nt][e] *= al;
+#pragma unroll
+                        for (int mt = 0; mt < D / 16; ++mt) {
+                            o[mt][nt][e] *= al;
+                            o[mt][nt][2 + e] *= al;
+                        }
+                    }
+            }
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float n0 = mr[nt][0] == -INFINITY ? 0.f : mr[nt][0], n1 = mr[nt][1] == -INFINITY ? 0.f : mr[nt][1];
+                pb[nt][0] = turn8x8(Half2<T>::pack(tc::ex2_approx(sc[nt][0] - n0), tc::ex2_approx(sc[nt][1] - n1)));
+                pb[nt][1] = turn8x8(Half2<T>::pack(tc::ex2_approx(sc[nt][2] - n0), tc::ex2_approx(sc[nt][3] - n1)));
+            }
+            const uint32_t one[4] = {Half2<T>::ones, Half2<T>::ones, Half2<T>::ones, Half2<T>::ones};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) Half2<T>::mma(ls[nt], one, pb[nt][0], pb[nt][1]);
+            {
+                const int r = (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+                for (int mt = 0; mt < D / 16; ++mt) {
+                    uint32_t f[4];
+                    ldm4t(f, va + (uint32_t)(r * D * 2 + (((mt * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4)));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) Half2<T>::mma(o[mt][nt], f, pb[nt][0], pb[nt][1]);
+                }
+            }
+        }
+
+        // ---- merge the warps' partials through the ring's memory
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+        __syncthreads();
+        float *om = reinterpret_cast<float *>(psm);                    // [PW][QR][OP]
+        float *mm = om + PW * S::QR * S::OP;                           // [PW][QR] max, then sums
+        float *lm = mm + PW * S::QR;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = nt * 8 + 2 * t + e;
+                float *dst = om + (warp * S::QR + c) * S::OP + g;
+#pragma unroll
+                for (int mt = 0; mt < D / 16; ++mt) {
+                    dst[mt * 16] = o[mt][nt][e];
+                    dst[mt * 16 + 8] = o[mt][nt][2 + e];
+                }
+                if (g == 0) {
+                    mm[warp * S::QR + c] = mr[nt][e];
+                    lm[warp * S::QR + c] = ls[nt][e];
+                }
+            }
+        __syncthreads();
+        const bool direct = whole && !force_partial;
+        // slots in order of (item, CTA): unique, since a piece starts a new item or a new CTA
+        const size_t slot = item + blockIdx.x;
+        for (int w = threadIdx.x; w < nq * (D / 4); w += PT) {
+            const int r = w / (D / 4), d = (w % (D / 4)) * 4;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < PW; ++i) mx = fmaxf(mx, mm[i * S::QR + r]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
+#pragma unroll
+            for (int i = 0; i < PW; ++i) {
+                const float mi = mm[i * S::QR + r];
+                const float f = weight_of(mi, lm[i * S::QR + r], mx);
+                const float4 y = *reinterpret_cast<const float4 *>(om + (i * S::QR + r) * S::OP + d);
+                l += f * lm[i * S::QR + r];
+                acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
+            }
+            if (direct) {
+                const int rr = qt * S::QR + r, m = t0 + rr / G;
+                if (__ldg(a.trow + m) < 0) continue;
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+                uint2 y;
+                y.x = Half2<T>::pack(acc.x * inv, acc.y * inv);
+                y.y = Half2<T>::pack(acc.z * inv, acc.w * inv);
+                *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr % G) * D + d) = y;
+            } else {
+                *reinterpret_cast<float4 *>(o_part + (slot * S::QR + r) * D + d) = acc;
+                if (d == 0) *reinterpret_cast<float2 *>(ml_part + (slot * S::QR + r) * 2) = make_float2(mx, l);
+            }
+        }
+        // the CTA that holds an item's first unit says where its pieces are
+        if (ua == 0 && threadIdx.x == 0) {
+            const int last = (int)(((ib + gu) * C - 1) / U);
+            meta[item] = direct ? make_int2(0, -2) : make_int2(blockIdx.x, last);
+        }
+        __syncthreads();   // the ring is filled again
+    }
+}
+
+// Merge an item's pieces (and, after a shared prefix, the prefix's splits):
+// thread = 8 features of a query row; pieces in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+attn_join(const PagedKV kv, const PagedQuery a, int QR, const float *__restrict__ o_part,
+          const float *__restrict__ ml_part, const int2 *__restrict__ meta, const PrefixPartials pre) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int Hq = a.n_heads, G = Hq / kv.n_kv;
+    const int qts = (a.qg * G + QR - 1) / QR, per_group = kv.n_kv * qts;
+    const size_t item = blockIdx.x;
+    const int grp = (int)(item / per_group), x = (int)(item % per_group), h = x / qts, qt = x - h * qts;
+    const int2 mt = meta[item];
+    if (mt.y < 0 && pre.splits == 0) return;   // written already
+    const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
+    const int nq = min(QR, ntok * G - qt * QR);
+    const int n_own = mt.y >= 0 ? mt.y - mt.x + 1 : 0, n = n_own + pre.splits;
+    constexpr int PB = 4;   // pieces whose loads are in flight together
+    for (int w = threadIdx.x; w < nq * (D / 8); w += blockDim.x) {
+        const int r = w / (D / 8), d = (w % (D / 8)) * 8;
+        const int rr = qt * QR + r, m = t0 + rr / G;
+        if (__ldg(a.trow + m) < 0) continue;
+        float acc[8], l = 0.f, mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+        for (int p0 = 0; p0 < n; p0 += PB) {
+            float2 ml[PB];
+            float4 va[PB], vb[PB];
+#pragma unroll
+            for (int k = 0; k < PB; ++k) {
+                ml[k] = make_float2(-INFINITY, 0.f);
+                va[k] = vb[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int p = p0 + k;
+                if (p < n) {
+                    size_t at;
+                    const float *os, *ms;
+                    if (p < n_own) {
+                        at = (item + mt.x + p) * QR + r;
+                        os = o_part; ms = ml_part;
+                    } else {
+                        at = ((size_t)(p - n_own) * kv.n_kv + h) * ((size_t)a.M * G) + (size_t)t0 * G + rr;
+                        os = pre.o; ms = pre.ml;
+                    }
+                    ml[k] = *reinterpret_cast<const float2 *>(ms + at * 2);
+                    va[k] = *reinterpret_cast<const float4 *>(os + at * D + d);
+                    vb[k] = *reinterpret_cast<const float4 *>(os + at * D + d + 4);
+                }
+            }
+            float mb = mx;
+#pragma unroll
+            for (int k = 0; k < PB; ++k) mb = fmaxf(mb, ml[k].x);
+            if (mx != -INFINITY && mx != mb) {
+                const float f = tc::ex2_approx(mx - mb);
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] *= f;
+            }
+            mx = mb;
+#pragma unroll
+            for (int k = 0; k < PB; ++k) {
+                const float f = weight_of(ml[k].x, ml[k].y, mb);
+                l += f * ml[k].y;
+                acc[0] += f * va[k].x; acc[1] += f * va[k].y; acc[2] += f * va[k].z; acc[3] += f * va[k].w;
+                acc[4] += f * vb[k].x; acc[5] += f * vb[k].y; acc[6] += f * vb[k].z; acc[7] += f * vb[k].w;
+            }
+        }
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        uint4 y;
+        y.x = Half2<T>::pack(acc[0] * inv, acc[1] * inv);
+        y.y = Half2<T>::pack(acc[2] * inv, acc[3] * inv);
+        y.z = Half2<T>::pack(acc[4] * inv, acc[5] * inv);
+        y.w = Half2<T>::pack(acc[6] * inv, acc[7] * inv);
+        *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr % G) * D + d) = y;
+    }
+}
+
+// query rows of an item: the n8 tiles that hold the group's rows, four at most
+int paged_nt(int qg, int G) { return std::min(4, (qg * G + 7) / 8); }
+
+struct Scratch {
+    size_t items, slots, ml_at, meta_at, bytes;
+};
+Scratch scratch_of(int M, int qg, int n_heads, int n_kv, int D, int sm_count) {
+    const int G = n_heads / n_kv, QR = paged_nt(qg, G) * 8;
+    const size_t groups = (M + qg - 1) / qg, qts = ((size_t)qg * G + QR - 1) / QR;
+    Scratch s;
+    s.items = groups * n_kv * qts;
+    s.slots = s.items + (size_t)sm_count * CTAS_PER_SM;
+    s.ml_at = s.slots * QR * D * 4;
+    s.meta_at = s.ml_at + ((s.slots * QR * 8 + 255) & ~(size_t)255);
+    s.bytes = s.meta_at + s.items * sizeof(int2);
+    return s;
+}
+
+template <typename T, int D, int NT>
+cudaError_t launch_main(const PagedKV &kv, const PagedQuery &q, int key_begin, bool partial, const Scratch &s, char *ws,
+                        int grid, cudaStream_t st) {
+    using P = PagedShape<D, NT>;
+    static bool attr[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!attr[dev & 63]) {
+        const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<T, D, NT>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, P::SMEM);
+        if (e != cudaSuccess) return e;
+        attr[dev & 63] = true;
+    }
+    return launch_pdl(paged_attn_kernel<T, D, NT>, dim3(grid), dim3(PT), (size_t)P::SMEM, st, kv, q, key_begin,
+                      partial ? 1 : 0, reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + s.ml_at),
+                      reinterpret_cast<int2 *>(ws + s.meta_at));
+}
+
+template <typename T, int D>
+cudaError_t run(const PagedKV &kv, const PagedQuery &q, int key_begin, const PrefixPartials &pre, char *ws,
+                int sm_count, cudaStream_t st) {
+    const int G = q.n_heads / kv.n_kv, NT = paged_nt(q.qg, G);
+    const Scratch s = scratch_of(q.M, q.qg, q.n_heads, kv.n_kv, D, sm_count);
+    const int grid = sm_count * CTAS_PER_SM;
+    const bool partial = pre.splits > 0;
+    cudaError_t e;
+    switch (NT) {
+        case 1: e = launch_main<T, D, 1>(kv, q, key_begin, partial, s, ws, grid, st); break;
+        case 2: e = launch_main<T, D, 2>(kv, q, key_begin, partial, s, ws, grid, st); break;
+        case 3: e = launch_main<T, D, 3>(kv, q, key_begin, partial, s, ws, grid, st); break;
+        default: e = launch_main<T, D, 4>(kv, q, key_begin, partial, s, ws, grid, st); break;
+    }
+    if (e != cudaSuccess) return e;
+    const int threads = std::min(256, (NT * 8 * (D / 8) + 31) / 32 * 32);
+    return launch_pdl(attn_join<T, D>, dim3((unsigned)s.items), dim3(threads), 0, st, kv, q, NT * 8,
+                      (const float *)ws, (const float *)(ws + s.ml_at), (const int2 *)(ws + s.meta_at), pre);
+}
+
+}  // namespace
+
+size_t paged_attn_scratch(int M, int qg, int n_heads, int n_kv, int D, int sm_count) {
+    return scratch_of(M, qg, n_heads, n_kv, D, sm_count).bytes;
+}
+
+cudaError_t paged_attn(const PagedKV &kv, const PagedQuery &q, int key_begin, const PrefixPartials &pre, void *scratch,
+                       int sm_count, cudaStream_t st) {
+    char *ws = static_cast<char *>(scratch);
+    if (kv.D == 128)
+        return kv.bf16 ? run<__nv_bfloat16, 128>(kv, q, key_begin, pre, ws, sm_count, st)
+                       : run<__half, 128>(kv, q, key_begin, pre, ws, sm_count, st);
+    return kv.bf16 ? run<__nv_bfloat16, 64>(kv, q, key_begin, pre, ws, sm_count, st)
+                   : run<__half, 64>(kv, q, key_begin, pre, ws, sm_count, st);
+}
+
+}  // namespace mlxcat

@@ -21,6 +21,7 @@
 #include "../../include/mlxcat_cuda.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "paged.h"
 
 using namespace mlxcat;
 
@@ -256,6 +257,22 @@ int op_err(int code, const char *fmt, ...) {
     g_op_err = buf;
     return code;
 }
+
+}  // namespace
+
+namespace mlxcat {
+int op_error(int code, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_op_err = buf;
+    return code;
+}
+}  // namespace mlxcat
+
+namespace {
 
 #define CK(ctx_, expr)                                                                      \
     do {                                                                                    \

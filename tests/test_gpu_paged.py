@@ -1,0 +1,643 @@
+"""The paged-cache operators on the GPU against their formulas in 64 bits.
+
+Tolerances, per element, from the arithmetic (u = eps / 2 of the output type):
+* append: the result rounded once (u |y|) and a few fp32 operations before it:
+  the sum of D squares moves the norm by at most D 2^-25 relatively, the angle's
+  fraction and sin / cos by 2^-22, the rotation's products by 3 * 2^-24; all of it
+  stays below 2^-16 (|a| + |b|) for D = 128.
+* attention: every weight is rounded once to the type (u, in the sum of the
+  weights as well), its score carries the fp32 dot product's error e = 2 D 2^-24
+  |q| |k| scale (2: the tensor cores truncate) and 2^-21 of the exponential, and
+  the result is rounded once.  With A = sum w |v|, the error is at most
+  u |y| + 2 A (u + e + 2^-21).  fp16 weights below 2^-14 of the largest have an
+  absolute error of 2^-25 each instead: n 2^-25 max|v| / sum 2^(z - max).
+"""
+import ctypes as C
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+from mlxcat_b200 import _abi as A  # noqa: E402
+
+L = A.lib()
+DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+CODE = {"f16": A.F16, "bf16": A.BF16, "f32": A.F32}
+NAN = float("nan")
+
+
+def ptr(t):
+    return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def stream():
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def half_step(dt):
+    return torch.finfo(DT[dt]).eps / 2
+
+
+class Paged:
+    """A cache of NaN pages, [page][head][token][d] or [page][token][head][d]."""
+
+    def __init__(self, hk, d, ps, n_pages, dt, table, nhd=False, fill=NAN):
+        shape = (n_pages, ps, hk, d) if nhd else (n_pages, hk, ps, d)
+        self.k = torch.full(shape, fill, dtype=DT[dt], device="cuda")
+        self.v = torch.full(shape, fill, dtype=DT[dt], device="cuda")
+        self.table = table if torch.is_tensor(table) else ints(table)
+        self.ps, self.hk, self.d, self.nhd = ps, hk, d, nhd
+        strides = (ps * hk * d, d, hk * d) if nhd else (ps * hk * d, ps * d, d)
+        self.c = A.PagedKVC(self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(), *strides, CODE[dt], n_pages, ps, hk, d,
+                            *self.table.shape)
+
+    def view(self, x):
+        return x.transpose(1, 2) if self.nhd else x          # [page][head][token][d]
+
+    def put(self, row, k, v, start=0):
+        """k, v [n, hk, d] at positions start.. of a row."""
+        pos = torch.arange(start, start + k.shape[0], device="cuda")
+        page = self.table[row, pos // self.ps].long()
+        self.view(self.k)[page, :, pos % self.ps] = k
+        self.view(self.v)[page, :, pos % self.ps] = v
+
+    def row(self, row, n):
+        pos = torch.arange(n, device="cuda")
+        page = self.table[row, pos // self.ps].long()
+        return self.view(self.k)[page, :, pos % self.ps], self.view(self.v)[page, :, pos % self.ps]
+
+
+def tables(lens, ps, spare=2, seed=0, lead=()):
+    """Shuffled page tables; entries past a row's end are -1.  lead: pages every row starts with."""
+    need = [max(0, math.ceil((n - len(lead) * ps) / ps)) for n in lens]
+    ids = torch.randperm(sum(need) + spare + len(lead), generator=torch.Generator().manual_seed(seed))
+    lead_ids, ids = ids[:len(lead)], ids[len(lead):]
+    t = torch.full((len(lens), len(lead) + max(1, max(need))), -1, dtype=torch.int32)
+    t[:, :len(lead)] = lead_ids
+    at = 0
+    for r, n in enumerate(need):
+        t[r, len(lead):len(lead) + n] = ids[at:at + n]
+        at += n
+    return t.cuda(), sum(need) + spare + len(lead)
+
+
+def attend64(q, k, v, limit, scale=None):
+    """q [n, h, d], k, v [keys, hk, d]; query i sees keys 0..limit[i].  Returns the result and the
+    tolerance's parts in 64 bits: A = sum w |v|, and the sum of 2^(z - max)."""
+    n, h, d = q.shape
+    g = h // k.shape[1]
+    if k.shape[0] == 0:
+        z = torch.zeros((n, h, d), dtype=torch.float64, device="cuda")
+        return z, z, torch.ones((n, h, 1), dtype=torch.float64, device="cuda")
+    kk, vv = k.double().repeat_interleave(g, 1), v.double().repeat_interleave(g, 1)
+    s = torch.einsum("nhd,khd->nhk", q.double(), kk) * (scale or 1 / math.sqrt(d))
+    seen = (torch.arange(k.shape[0], device="cuda")[None, :] <= limit[:, None])[:, None, :]
+    s = s.masked_fill(~seen, float("-inf"))
+    top = s.amax(-1, keepdim=True).clamp(min=-1e300)
+    e = torch.exp(s - top)
+    tot = e.sum(-1, keepdim=True)
+    w = e / tot.clamp(min=1e-300)
+    return torch.einsum("nhk,khd->nhd", w, vv), torch.einsum("nhk,khd->nhd", w, vv.abs()), tot.clamp(min=1.0)
+
+
+def check(got, ref, dt, q, k, v, scale=None):
+    y, a, tot = ref
+    d = q.shape[-1]
+    assert torch.isfinite(got.double()).all()
+    e = 0.0 if k.shape[0] == 0 else (2 * d * 2.0 ** -24 * q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max() *
+                                     (scale or 1 / math.sqrt(d))).item()
+    u = half_step(dt)
+    tol = u * y.abs() + 2 * a * (u + e + 2.0 ** -21) + 1e-7
+    if dt == "f16" and k.shape[0]:
+        tol = tol + k.shape[0] * 2.0 ** -25 * v.double().abs().max() / tot
+    worst = ((got.double() - y).abs() / tol).max().item()
+    assert worst <= 1.0, worst
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rnd(shape, g, dt, scale=1.0):
+    return (torch.randn(shape, device="cuda", generator=g) * scale).to(DT[dt])
+
+
+# ------------------------------------------------------------------------------------------------- append
+def rope_plan(rd, layout, theta=500000.0, kind=0):
+    r, s = A.RopeC(), A.RopeScalingC(kind, 8192, 8.0, 1.0, 4.0, 32.0, 1.0, 0.0)
+    A.check(L.mlxcat_rope_init(C.byref(r), rd, layout, theta, C.byref(s)))
+    return r
+
+
+def append(cache, plan, q, k, v, src, trow, tpos, q_out, qn=None, kn=None, eps=1e-6, err=None, heads=None):
+    return L.mlxcat_op_rope_append(C.byref(cache.c), plan and C.byref(plan), ptr(q), ptr(k), ptr(v), CODE[src], q.stride(0) if q is not None else 0,
+                                   k.stride(0), v.stride(0), k.shape[0], heads if heads is not None else (q.shape[1] // cache.d if q is not None else 0),
+                                   ptr(qn), ptr(kn), eps, ptr(trow), ptr(tpos), ptr(q_out), ptr(err), stream())
+
+
+def turned64(x, pos, plan, w, eps=1e-6):
+    """x [m, heads, d] -> normalised and rotated in 64 bits, and |a| + |b| of each pair."""
+    x = x.double()
+    if w is not None:
+        x = x / ((x * x).mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    size = x.abs()
+    if plan is not None:
+        rd = plan.rotary_dim
+        turns = torch.tensor(plan.turns[:rd // 2], dtype=torch.float64, device="cuda")
+        ang = (pos.double()[:, None] * turns)[:, None, :] * (2 * math.pi)
+        z = torch.arange(rd // 2, device="cuda")
+        ia, ib = (z, z + rd // 2) if plan.layout == A.ROPE_HALF else (2 * z, 2 * z + 1)
+        a, b = x[..., ia], x[..., ib]
+        x = x.clone()
+        x[..., ia] = plan.mscale * (a * ang.cos() - b * ang.sin())
+        x[..., ib] = plan.mscale * (b * ang.cos() + a * ang.sin())
+        size = size.clone()
+        size[..., ia] = size[..., ib] = plan.mscale * (a.abs() + b.abs())
+    return x, size
+
+
+def near(got, y, size, dt):
+    tol = half_step(dt) * y.abs() + 2.0 ** -16 * size + 1e-7
+    worst = ((got.double() - y).abs() / tol).max().item()
+    assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("d,h,hk,dt,src,rd,layout,kind,norm,ps,nhd", [
+    (64, 8, 2, "f16", "f16", 64, 0, 0, False, 16, False),
+    (128, 32, 8, "f16", "f32", 128, 0, 2, False, 64, True),
+    (128, 32, 8, "bf16", "bf16", 128, 1, 3, True, 256, False),
+    (128, 10, 2, "bf16", "f32", 32, 0, 1, True, 8, False),
+    (64, 3, 1, "f16", "bf16", 20, 0, 0, True, 32, True),      # half of the rotary width no multiple of 8
+    (64, 5, 5, "bf16", "f16", 6, 1, 0, False, 8, False),
+    (128, 1, 1, "f16", "f16", 2, 0, 0, False, 128, False),
+    (128, 4, 4, "f16", "f32", 0, 0, 0, True, 16, False),      # no rotation
+])
+@pytest.mark.parametrize("t", [1, 37])
+def test_append(d, h, hk, dt, src, rd, layout, kind, norm, ps, nhd, t):
+    g = gen(d + h + t)
+    past = [0, 5, 130]
+    table, n_pages = tables([p + t for p in past], ps)
+    cache = Paged(hk, d, ps, n_pages, dt, table, nhd, fill=7.0)
+    m = 3 * t
+    x = rnd((m, (h + 2 * hk) * d + 8), g, src, 2.0)           # a fused projection with padding behind it
+    q, k, v = x[:, :h * d], x[:, h * d:(h + hk) * d], x[:, (h + hk) * d:(h + 2 * hk) * d]
+    trow = ints([r for r in range(3) for _ in range(t)])
+    tpos = ints([past[r] + j for r in range(3) for j in range(t)])
+    trow[1 if t > 1 else 0] = -1                              # a padding token
+    plan = rope_plan(rd, layout, kind=kind) if rd else None
+    qn = kn = None
+    if norm:
+        qn, kn = 1 + 0.3 * torch.randn(d, device="cuda", generator=g), 1 + 0.3 * torch.randn(d, device="cuda", generator=g)
+    q_out = torch.full((m, h, d), 9.0, dtype=DT[dt], device="cuda")
+    err = ints([0])
+    A.check(append(cache, plan, q, k, v, src, trow, tpos, q_out, qn, kn, err=err))
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    on = trow >= 0
+    y, size = turned64(q.reshape(m, h, d), tpos, plan, qn)
+    near(q_out[on], y[on], size[on], dt)
+    assert (q_out[~on] == 9.0).all()
+    y, size = turned64(k.reshape(m, hk, d), tpos, plan, kn)
+    page, off = table[trow.long().clamp(min=0), (tpos // ps).long()].long()[on], (tpos % ps).long()[on]
+    near(cache.view(cache.k)[page, :, off], y[on], size[on], dt)
+    assert torch.equal(cache.view(cache.v)[page, :, off], v.reshape(m, hk, d)[on].to(DT[dt]))
+    for c in (cache.k, cache.v):                              # nothing else was written
+        w = cache.view(c).clone()
+        w[page, :, off] = 7.0
+        assert (w == 7.0).all()
+
+
+def test_append_far_positions():
+    """Positions up to 2^30: the angle keeps its fraction."""
+    ps, d = 65536, 128
+    pos = [0, 1, 65535, 65536, 10 ** 6 + 1, 2 ** 24 + 3, 2 ** 30 - 1]
+    pages = sorted({p // ps for p in pos})
+    table = torch.full((1, 2 ** 30 // ps), -1, dtype=torch.int32)
+    for i, p in enumerate(pages):
+        table[0, p] = i
+    cache = Paged(1, d, ps, len(pages), "f16", table.cuda(), fill=0.0)
+    g = gen(3)
+    q, k = rnd((len(pos), 2 * d), g, "f32"), rnd((len(pos), d), g, "f32")
+    q_out = torch.zeros((len(pos), 2, d), dtype=torch.float16, device="cuda")
+    plan = rope_plan(d, A.ROPE_HALF, 10000.0)
+    A.check(append(cache, plan, q, k, k, "f32", ints([0] * len(pos)), ints(pos), q_out))
+    y, size = turned64(q.view(-1, 2, d), torch.tensor(pos, device="cuda"), plan, None)
+    near(q_out, y, size, "f16")
+
+
+def test_append_out_of_range():
+    d, ps = 64, 16
+    table = ints([[0, 1], [2, 99]])
+    for trow, tpos, bad in [(0, 32, True), (0, -1, True), (2, 0, True), (1, 16, True), (1, 15, False)]:
+        cache = Paged(2, d, ps, 3, "f16", table, fill=5.0)
+        x = torch.ones((1, 2 * d), dtype=torch.float16, device="cuda")
+        q_out = torch.zeros((1, 2, d), dtype=torch.float16, device="cuda")
+        err = ints([0])
+        A.check(append(cache, None, x, x, x, "f16", ints([trow]), ints([tpos]), q_out, err=err))
+        assert (err.item() != 0) == bad
+        assert bool((cache.k == 5.0).all()) == bad
+        assert (q_out == 1).all()
+        A.check(append(cache, None, x, x, x, "f16", ints([trow]), ints([tpos]), q_out))   # err may be NULL
+
+
+def test_append_keys_only():
+    cache = Paged(2, 64, 16, 1, "bf16", ints([[0]]), fill=0.0)
+    x = rnd((3, 128), gen(1), "bf16")
+    A.check(append(cache, None, None, x, x, "bf16", ints([0, 0, 0]), ints([0, 5, 15]), None))
+    k, v = cache.row(0, 16)
+    assert torch.equal(k[[0, 5, 15]].reshape(3, 128), x) and torch.equal(v, k)
+
+
+# ---------------------------------------------------------------------------------------- paged attention
+def fill_rows(cache, lens, g, dt, shared=0):
+    for r, n in enumerate(lens):
+        a = shared if r else 0
+        if n > a:
+            cache.put(r, rnd((n - a, cache.hk, cache.d), g, dt), rnd((n - a, cache.hk, cache.d), g, dt), a)
+
+
+def paged(cache, q, qg, trow, tpos, out, prefix=None, scale=0.0, err=None, ws=None, st=None):
+    m, h, d = q.shape
+    size = (L.mlxcat_op_paged_attention_workspace(m, qg, h, cache.hk, d) if prefix is None else
+            L.mlxcat_op_shared_prefix_attention_workspace(m, qg, h, cache.hk, d, prefix))
+    ws = torch.full((size,), 0xff, dtype=torch.uint8, device="cuda") if ws is None else ws
+    rest = (ptr(q), m, qg, h, scale, ptr(trow), ptr(tpos), ptr(out), ptr(ws), size, ptr(err), st or stream())
+    if prefix is None:
+        return L.mlxcat_op_paged_attention(C.byref(cache.c), *rest)
+    return L.mlxcat_op_shared_prefix_attention(C.byref(cache.c), prefix, *rest)
+
+
+def check_rows(cache, q, qg, trow, tpos, out, dt, scale=None):
+    for i in range(q.shape[0]):
+        r, p = trow[i].item(), tpos[i].item()
+        if r < 0:
+            assert (out[i] == 9.0).all()
+            continue
+        if p < 0:
+            assert (out[i] == 0).all()
+            continue
+        k, v = cache.row(r, p + 1)
+        check(out[i:i + 1], attend64(q[i:i + 1], k, v, tpos[i:i + 1].long(), scale), dt, q[i:i + 1], k, v, scale)
+
+
+LENS = [1, 2, 63, 64, 65, 127, 300, 1027]
+
+
+@pytest.mark.parametrize("h,hk,d,dt,qg,ps,nhd", [
+    (8, 2, 64, "f16", 1, 16, False), (32, 8, 128, "f16", 5, 64, False), (32, 8, 128, "bf16", 1, 256, True), (64, 8, 128, "bf16", 4, 8, False),
+    (10, 2, 128, "f16", 3, 32, True), (4, 4, 64, "bf16", 1, 8, False), (40, 1, 64, "f16", 2, 128, False), (32, 4, 128, "bf16", 8, 16, False),
+    (3, 1, 128, "f16", 1, 1024, False), (12, 4, 64, "f16", 7, 32, False)])
+def test_paged_attention(h, hk, d, dt, qg, ps, nhd):
+    g = gen(h + d + qg)
+    lens = [n + qg - 1 for n in LENS]
+    table, n_pages = tables(lens, ps)
+    cache = Paged(hk, d, ps, n_pages, dt, table, nhd)       # what no row holds is NaN
+    fill_rows(cache, lens, g, dt)
+    trow = ints([r for r in range(len(lens)) for _ in range(qg)])
+    tpos = ints([n - qg + j for n in lens for j in range(qg)])
+    q = rnd((len(trow), h, d), g, dt)
+    out = torch.full_like(q, 9.0)
+    err = ints([0])
+    A.check(paged(cache, q, qg, trow, tpos, out, err=err))
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    check_rows(cache, q, qg, trow, tpos, out, dt)
+    again = torch.full_like(q, 9.0)
+    A.check(paged(cache, q, qg, trow, tpos, again))
+    assert torch.equal(out, again)                           # no order of arrival in the result
+
+
+def test_paged_attention_many_splits_and_many_rows():
+    for lens, h, hk in (([20000], 8, 1), ([5] * 300 + [900], 8, 2)):
+        g = gen(len(lens))
+        table, n_pages = tables(lens, 16)
+        cache = Paged(hk, 128, 16, n_pages, "f16", table)
+        fill_rows(cache, lens, g, "f16")
+        trow, tpos = ints(list(range(len(lens)))), ints([n - 1 for n in lens])
+        q = rnd((len(lens), h, 128), g, "f16")
+        out = torch.full_like(q, 9.0)
+        A.check(paged(cache, q, 1, trow, tpos, out))
+        check_rows(cache, q, 1, trow, tpos, out, "f16")
+
+
+@pytest.mark.parametrize("prefix", [None, 32])
+def test_paged_attention_empty_and_padding(prefix):
+    """Rows without keys give zeros, padding stays as it was, groups end in padding, a short last group."""
+    qg, ps, dt, h, hk, d = 3, 16, "bf16", 8, 2, 64
+    lens = [40, 0, 50, 33, 36]
+    table, n_pages = tables(lens, ps, lead=(0, 0) if prefix else ())
+    cache = Paged(hk, d, ps, n_pages, dt, table)
+    g = gen(5)
+    fill_rows(cache, lens, g, dt, shared=prefix or 0)
+    if prefix:
+        table[1] = table[0]
+    trow = ints([0, 0, 0, 1, 1, 1, 2, 2, -1, -1, -1, -1, 3, 3, 3, 4])
+    tpos = ints([37, 38, 39, -1, -1, -1, 48, 49, 0, 7, 8, 9, -1, 0, 32, 35])
+    q = rnd((len(trow), h, d), g, dt)
+    out = torch.full_like(q, 9.0)
+    A.check(paged(cache, q, qg, trow, tpos, out, prefix))
+    check_rows(cache, q, qg, trow, tpos, out, dt)
+
+
+@pytest.mark.parametrize("prefix", [None, 16])
+def test_paged_attention_out_of_range(prefix):
+    """Rows, positions and pages outside the cache set the flag; nothing is read there."""
+    ps, h, hk, d = 16, 8, 2, 64
+    for trow, tpos, table in ([5, 3, ints([[0, 1]])], [0, 32, ints([[0, 1]])], [0, 0x7fffffff, ints([[0, 1]])], [0, 20, ints([[0, 44]])],
+                              [0, 20, ints([[-7, 1]])]):
+        cache = Paged(hk, d, ps, 2, "f16", table, fill=0.5)
+        q, err = rnd((1, h, d), gen(1), "f16"), ints([0])
+        out = torch.full_like(q, 9.0)
+        A.check(paged(cache, q, 1, ints([trow]), ints([tpos]), out, prefix, err=err))
+        torch.cuda.synchronize()
+        assert err.item() != 0 and torch.isfinite(out).all()
+        A.check(paged(cache, q, 1, ints([trow]), ints([tpos]), out, prefix))
+
+
+def test_paged_attention_scale_and_large_scores():
+    """A scale of its own; scores far apart, so that the running maximum moves often."""
+    lens, g = [700, 90], gen(8)
+    table, n_pages = tables(lens, 32)
+    cache = Paged(2, 64, 32, n_pages, "bf16", table)
+    fill_rows(cache, lens, g, "bf16")
+    for r, n in enumerate(lens):
+        k, v = cache.row(r, n)
+        cache.put(r, k * torch.linspace(0.1, 6.0, n, device="cuda").to(k.dtype)[:, None, None], v)
+    trow, tpos = ints([0, 1]), ints([699, 89])
+    q = rnd((2, 8, 64), g, "bf16", 3.0)
+    for prefix in (None, 64):
+        if prefix:
+            table[1, :2] = table[0, :2]
+        out = torch.full_like(q, 9.0)
+        A.check(paged(cache, q, 1, trow, tpos, out, prefix, scale=0.3))
+        check_rows(cache, q, 1, trow, tpos, out, "bf16", 0.3)
+
+
+def test_paged_attention_far_pages():
+    """Pages whose elements lie past 2^32."""
+    ps, hk, d = 256, 2, 128
+    n_pages = 2 ** 32 // (ps * hk * d) + 3
+    k, v = (torch.empty((n_pages, hk, ps, d), dtype=torch.float16, device="cuda") for _ in range(2))
+    table = ints([[n_pages - 1, 0, n_pages - 2]])
+    cache = Paged(hk, d, ps, 1, "f16", table)
+    cache.k, cache.v = k, v
+    cache.c.k, cache.c.v, cache.c.n_pages = k.data_ptr(), v.data_ptr(), n_pages
+    g = gen(2)
+    x = rnd((700, 4 * hk * d), g, "f32")
+    q_out = torch.zeros((700, 2 * hk, d), dtype=torch.float16, device="cuda")
+    A.check(append(cache, None, x[:, :2 * hk * d], x[:, 2 * hk * d:3 * hk * d], x[:, 3 * hk * d:], "f32", ints([0] * 700),
+                   ints(list(range(700))), q_out))
+    kk, vv = cache.row(0, 700)
+    assert torch.equal(kk.reshape(700, -1), x[:, 2 * hk * d:3 * hk * d].half()) and torch.equal(vv.reshape(700, -1), x[:, 3 * hk * d:].half())
+    for prefix in (None, 512):
+        out = torch.full((1, 4, d), 9.0, dtype=torch.float16, device="cuda")
+        A.check(paged(cache, q_out[:1].contiguous(), 1, ints([0]), ints([699]), out, prefix))
+        check_rows(cache, q_out[:1], 1, ints([0]), ints([699]), out, "f16")
+
+
+# ------------------------------------------------------------------------------------------ shared prefix
+@pytest.mark.parametrize("h,hk,d,dt,qg,ps,prefix,rows,nhd", [
+    (8, 2, 64, "f16", 1, 16, 48, 3, False), (32, 8, 128, "bf16", 1, 256, 2048, 40, False), (32, 8, 128, "f16", 5, 64, 320, 9, True),
+    (32, 4, 128, "bf16", 4, 8, 2056, 20, False), (10, 2, 64, "bf16", 2, 32, 416, 30, True), (64, 1, 128, "f16", 1, 128, 1024, 5, False),
+    (4, 4, 128, "f16", 1, 16, 16, 1, False), (48, 16, 64, "f16", 3, 8, 136, 70, False)])
+def test_shared_prefix_attention(h, hk, d, dt, qg, ps, prefix, rows, nhd):
+    g = gen(h + d + rows)
+    own = [(1, 2, 63, 64, 65, 200)[r % 6] + qg - 1 for r in range(rows)]
+    lens = [prefix + n for n in own]
+    table, n_pages = tables(lens, ps, lead=(0,) * (prefix // ps))
+    cache = Paged(hk, d, ps, n_pages, dt, table, nhd)
+    fill_rows(cache, lens, g, dt, shared=prefix)
+    trow = [r for r in range(rows) for _ in range(qg)]
+    tpos = [n - qg + j for n in lens for j in range(qg)]
+    if rows > 4:                       # rows that end inside the prefix, padding first
+        tpos[-qg:] = [max(0, prefix // 2 - 3) + j for j in range(qg)]
+        tpos[-2 * qg:-qg] = list(range(qg))
+        trow[:qg] = [-1] * qg
+    trow, tpos = ints(trow), ints(tpos)
+    q = rnd((len(trow), h, d), g, dt)
+    out, err = torch.full_like(q, 9.0), ints([0])
+    A.check(paged(cache, q, qg, trow, tpos, out, prefix, err=err))
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    check_rows(cache, q, qg, trow, tpos, out, dt)
+    again = torch.full_like(q, 9.0)
+    A.check(paged(cache, q, qg, trow, tpos, again, prefix))
+    assert torch.equal(out, again)
+
+
+# ------------------------------------------------------------------------------------------------- packed
+def packed(q, k, v, cu_q, cu_k, causal, out, dt, scale=0.0, err=None):
+    return L.mlxcat_op_packed_attention(ptr(q), ptr(k), ptr(v), CODE[dt], q.stride(0), k.stride(0), v.stride(0), q.shape[0], k.shape[0],
+                                        ptr(cu_q), ptr(cu_k), len(cu_q) - 1, causal, q.shape[1], k.shape[1], q.shape[2], scale, ptr(out),
+                                        ptr(err), stream())
+
+
+def check_packed(q, k, v, cu_q, cu_k, causal, out, dt, scale=None):
+    cq, ck = cu_q.tolist(), cu_k.tolist()
+    for i in range(len(cq) - 1):
+        nq, nk = cq[i + 1] - cq[i], ck[i + 1] - ck[i]
+        if not nq:
+            continue
+        lim = torch.arange(nq, device="cuda") + nk - nq if causal else torch.full((nq,), nk - 1, device="cuda")
+        qq, kk, vv = q[cq[i]:cq[i + 1]], k[ck[i]:ck[i + 1]], v[ck[i]:ck[i + 1]]
+        o = out[cq[i]:cq[i + 1]]
+        assert (o[lim < 0] == 0).all()
+        check(o, attend64(qq, kk, vv, lim, scale), dt, qq, kk, vv, scale)
+
+
+@pytest.mark.parametrize("h,hk,d,dt", [(8, 2, 64, "f16"), (32, 8, 128, "bf16"), (32, 8, 128, "f16"), (10, 2, 128, "f16"), (4, 4, 64, "bf16"),
+                                       (33, 1, 64, "f16"), (64, 1, 128, "bf16"), (6, 2, 128, "bf16")])
+@pytest.mark.parametrize("lens,past,causal", [
+    ([1], [0], 1), ([1, 1, 1], [0, 5, 200], 1), ([3, 0, 77, 128, 1], [0, 9, 0, 0, 127], 1), ([257, 31, 640], [0, 300, 1], 1),
+    ([64, 129], [0, 63], 0), ([5, 130, 40], [-3, -70, -40], 1)])
+def test_packed_attention(h, hk, d, dt, lens, past, causal):
+    g = gen(h + d + sum(lens))
+    klens = [a + b for a, b in zip(lens, past)]
+    cu_q, cu_k = ints([0] + torch.tensor(lens).cumsum(0).tolist()), ints([0] + torch.tensor(klens).cumsum(0).tolist())
+    x = rnd((sum(lens), (h + 2) * d), g, dt)                   # strided queries
+    q = x.view(sum(lens), h + 2, d)[:, 1:h + 1]
+    k, v = rnd((max(1, sum(klens)), hk, d), g, dt), rnd((max(1, sum(klens)), hk, d), g, dt)
+    out = torch.full((sum(lens), h, d), 9.0, dtype=DT[dt], device="cuda")
+    err = ints([0])
+    if (q.data_ptr() & 15):
+        pytest.skip("unaligned slice")
+    A.check(packed(q, k, v, cu_q, cu_k, causal, out, dt, err=err))
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    check_packed(q, k, v, cu_q, cu_k, causal, out, dt)
+
+
+def test_packed_attention_keeps_sequences_apart():
+    """Non-finite keys and values of one sequence, or behind all, reach no other; tokens outside stay."""
+    lens, d, h, hk = [70, 33, 90], 128, 8, 2
+    for dt in ("f16", "bf16"):
+        g = gen(4)
+        q, k, v = rnd((230, h, d), g, dt), rnd((230, hk, d), g, dt), rnd((230, hk, d), g, dt)
+        cu = ints([10, 80, 113, 203])
+        for bad in (NAN, float("inf"), float("-inf")):
+            kb, vb = k.clone(), v.clone()
+            for x in (kb, vb):
+                x[:10] = bad
+                x[80:113] = bad
+                x[203:] = bad
+            out = torch.full((230, h, d), 9.0, dtype=DT[dt], device="cuda")
+            A.check(packed(q, kb, vb, cu, cu, 1, out, dt))
+            for a, b in ((10, 80), (113, 203)):
+                n = b - a
+                check(out[a:b], attend64(q[a:b], k[a:b], v[a:b], torch.arange(n, device="cuda")), dt, q[a:b], k[a:b], v[a:b])
+            assert (out[:10] == 9.0).all() and (out[203:] == 9.0).all()
+            assert not torch.isfinite(out[80:113].float()).any()
+
+
+def test_packed_attention_large_scores_and_scale():
+    g = gen(6)
+    q, k, v = rnd((700, 8, 64), g, "bf16", 3.0), rnd((700, 2, 64), g, "bf16"), rnd((700, 2, 64), g, "bf16")
+    k = k * torch.linspace(0.1, 6.0, 700, device="cuda").to(k.dtype)[:, None, None]
+    cu = ints([0, 700])
+    out = torch.full_like(q, 9.0)
+    A.check(packed(q, k, v, cu, cu, 1, out, "bf16", scale=0.3))
+    check_packed(q, k, v, cu, cu, 1, out, "bf16", 0.3)
+
+
+def test_packed_attention_bad_offsets_stay_inside():
+    """Offsets past the buffers are cut to them: finite results, nothing written outside the queries."""
+    g = gen(7)
+    q, k, v = rnd((40, 8, 64), g, "f16"), rnd((40, 2, 64), g, "f16"), rnd((40, 2, 64), g, "f16")
+    for cq, ck in (([0, 1000], [0, 1000]), ([-50, 20], [-9, 30]), ([30, 10, 60], [50, 2, 3]), ([0, 2 ** 31 - 1], [0, 2 ** 31 - 1])):
+        out = torch.full((48, 8, 64), 9.0, dtype=torch.float16, device="cuda")
+        A.check(packed(q, k, v, ints(cq), ints(ck), 1, out, "f16"))
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all() and (out[40:] == 9.0).all()
+
+
+# ------------------------------------------------------------------------------------ graphs and streams
+def test_graph_replay_and_two_streams():
+    """One capture of append + attention replayed on new lengths, and two streams with a workspace each."""
+    rows, h, hk, d, ps, dt = 4, 8, 2, 64, 16, "f16"
+    g = gen(9)
+    lens = [30, 17, 64, 200]
+    table, n_pages = tables([n + 8 for n in lens], ps)
+    cache = Paged(hk, d, ps, n_pages, dt, table)
+    fill_rows(cache, lens, g, dt)
+    trow, tpos = ints(list(range(rows))), ints(lens)
+    x = rnd((rows, (h + 2 * hk) * d), g, "f32")
+    q, k, v = x[:, :h * d], x[:, h * d:(h + hk) * d], x[:, (h + hk) * d:]
+    q_out, out = torch.zeros((rows, h, d), dtype=DT[dt], device="cuda"), torch.zeros((rows, h, d), dtype=DT[dt], device="cuda")
+    plan = rope_plan(d, A.ROPE_HALF)
+    ws = torch.empty(L.mlxcat_op_paged_attention_workspace(rows, 1, h, hk, d), dtype=torch.uint8, device="cuda")
+
+    def step():
+        A.check(append(cache, plan, q, k, v, "f32", trow, tpos, q_out))
+        A.check(paged(cache, q_out, 1, trow, tpos, out, ws=ws))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):
+        x.copy_(rnd(x.shape, g, "f32"))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_rows(cache, q_out, 1, trow, tpos, out, dt)
+        tpos += 1
+    outs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    tpos -= 1
+    torch.cuda.synchronize()
+    qs = [rnd((rows, h, d), g, dt) for _ in range(2)]
+    for s, qq in zip(streams, qs):
+        with torch.cuda.stream(s):
+            outs.append(torch.full_like(qq, 9.0))
+            for _ in range(20):
+                A.check(paged(cache, qq, 1, trow, tpos, outs[-1]))
+    torch.cuda.synchronize()
+    for qq, o in zip(qs, outs):
+        check_rows(cache, qq, 1, trow, tpos, o, dt)
+
+
+# -------------------------------------------------------------------------------------- a serving run
+@pytest.mark.parametrize("dt,d", [("f16", 128), ("bf16", 64)])
+def test_serving_run(dt, d):
+    """Admission of three prompts behind one shared instruction block, then verify steps of three tokens:
+    append + packed attention, append + paged / shared-prefix attention, against the dense formula on the
+    keys and values that the formula itself rotates."""
+    h, hk, ps, qg, prefix = 8, 2, 32, 3, 64
+    prompts = [70, 128, 33]                     # tokens after the shared block
+    rows, steps = 3, 4
+    g = gen(d)
+    lens = [prefix + p + qg * steps for p in prompts]
+    table, n_pages = tables(lens, ps, lead=(0, 0))
+    cache = Paged(hk, d, ps, n_pages, dt, table)
+    plan = rope_plan(d, A.ROPE_HALF)
+    qn, kn = (1 + 0.2 * torch.randn(d, device="cuda", generator=g) for _ in range(2))
+    width = (h + 2 * hk) * d
+    keys, vals = [None] * rows, [None] * rows   # what the formula has, rounded to the cache's type
+
+    def project(x, tpos):
+        m = x.shape[0]
+        q = turned64(x[:, :h * d].view(m, h, d), tpos, plan, qn)[0]
+        k = turned64(x[:, h * d:(h + hk) * d].view(m, hk, d), tpos, plan, kn)[0]
+        return q.to(DT[dt]), k.to(DT[dt]), x[:, (h + hk) * d:].view(m, hk, d).to(DT[dt])
+
+    def run_append(x, trow, tpos):
+        q_out = torch.zeros((x.shape[0], h, d), dtype=DT[dt], device="cuda")
+        A.check(append(cache, plan, x[:, :h * d], x[:, h * d:(h + hk) * d], x[:, (h + hk) * d:], "f32", trow, tpos, q_out, qn, kn))
+        return q_out
+
+    def loose(got, q, k, v, lim):
+        # the operands themselves are one rounding apart (2 u each way in q and k): scores differ by up to
+        # 4 u |q| |k| / sqrt(d), the values by u
+        y, a, _ = attend64(q, k, v, lim)
+        u = half_step(dt)
+        ds = 4 * u * (q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max()).item() / math.sqrt(d)
+        tol = u * y.abs() + 2 * a * (2 * u + math.expm1(2 * ds)) + 1e-6
+        assert ((got.double() - y).abs() <= tol).all()
+
+    x = rnd((prefix, width), g, "f32")          # the shared block, appended once
+    pos = torch.arange(prefix, device="cuda", dtype=torch.int32)
+    run_append(x, ints([0] * prefix), pos)
+    _, k0, v0 = project(x, pos)
+    xs = [rnd((p, width), g, "f32") for p in prompts]
+    x = torch.cat(xs)
+    trow = ints([r for r in range(rows) for _ in range(prompts[r])])
+    tpos = ints([prefix + j for r in range(rows) for j in range(prompts[r])])
+    q_out = run_append(x, trow, tpos)
+    kv = [cache.row(r, prefix + prompts[r]) for r in range(rows)]
+    k, v = torch.cat([a for a, _ in kv]), torch.cat([b for _, b in kv])
+    cu_q = ints([0] + torch.tensor(prompts).cumsum(0).tolist())
+    cu_k = ints([0] + (torch.tensor(prompts) + prefix).cumsum(0).tolist())
+    out = torch.zeros_like(q_out)
+    A.check(packed(q_out, k, v, cu_q, cu_k, 1, out, dt))
+    for r in range(rows):
+        a, b = cu_q[r].item(), cu_q[r + 1].item()
+        qq, kk, vv = project(xs[r], tpos[a:b])
+        keys[r], vals[r] = torch.cat([k0, kk]), torch.cat([v0, vv])
+        loose(out[a:b], qq, keys[r], vals[r], tpos[a:b].long())
+    at = [prefix + p for p in prompts]
+    for _ in range(steps):
+        x = rnd((rows * qg, width), g, "f32")
+        trow = ints([r for r in range(rows) for _ in range(qg)])
+        tpos = ints([at[r] + j for r in range(rows) for j in range(qg)])
+        q_out = run_append(x, trow, tpos)
+        o1, o2 = torch.zeros_like(q_out), torch.zeros_like(q_out)
+        A.check(paged(cache, q_out, qg, trow, tpos, o1))
+        A.check(paged(cache, q_out, qg, trow, tpos, o2, prefix))
+        for r in range(rows):
+            s = slice(r * qg, (r + 1) * qg)
+            qq, kk, vv = project(x[s], tpos[s])
+            keys[r], vals[r] = torch.cat([keys[r], kk]), torch.cat([vals[r], vv])
+            loose(o1[s], qq, keys[r], vals[r], tpos[s].long())
+            loose(o2[s], qq, keys[r], vals[r], tpos[s].long())
+            at[r] += qg
