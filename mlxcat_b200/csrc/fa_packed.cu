@@ -23,8 +23,8 @@
 // are zeroed in shared memory before the product, so what lies behind a
 // sequence (another prompt, an unwritten page, NaN) does not reach it.
 //
-// Warps: 0 TMA producer, 1 MMA issuer, 2 TMEM allocation, 4-7 softmax of tile
-// 0, 8-11 of tile 1.  Every wait is bounded; a timeout sets *err and an abort
+// Warps: 0 TMA producer, 1 and 3 MMA issuers of tiles 0 and 1, 2 TMEM
+// allocation, 4-7 softmax of tile 0, 8-11 of tile 1.  Every wait is bounded; a timeout sets *err and an abort
 // flag after which every role skips its work, the producer waits for its copies
 // and the issuer for what it committed, and the CTA frees TMEM.
 #include <cuda.h>
@@ -48,12 +48,14 @@ constexpr int KB = 128;                 // keys of a block
 constexpr int BOX = 128 * 128;          // [128 rows][64 features] swizzled
 constexpr int SLOTS = 5;                // K / V ring
 constexpr int THREADS = 384;
+constexpr int SB = 64;                  // keys of a score buffer: two per tile
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
-enum PkErr { PK_Q = 61, PK_KV, PK_FREE, PK_S, PK_P, PK_PV };
+enum PkErr { PK_Q = 61, PK_KV, PK_FREE, PK_S, PK_P, PK_PV, PK_ALIGN };
 
 struct Bars {
-    unsigned long long q_full, full[SLOTS], freed[SLOTS], s_full[2], p_full[2], pv_done[2], fin;
+    unsigned long long q_full, full[SLOTS], freed[SLOTS], skew, tail, fin[2];
+    unsigned long long s_full[2][2], p_full[2][2], pv_done[2][2];   // [tile][score buffer]
     uint32_t tmem;
     int abort;
 };
@@ -62,7 +64,8 @@ template <int D>
 struct Shape {
     static constexpr int HALVES = D / 64;
     static constexpr int TILE = HALVES * BOX;
-    static constexpr int SMEM = 1024 + (2 + SLOTS) * TILE + (int)sizeof(Bars);
+    static constexpr int SMEM = (2 + SLOTS) * TILE + (int)sizeof(Bars);
+    static_assert(SMEM <= 227 * 1024, "two Q tiles and the ring must fit one CTA");
 };
 
 struct Args {
@@ -86,10 +89,65 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
         : "memory");
 }
 
+// one lane of the warp, the same each time
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float lo2(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi2(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t exp2_unit(uint64_t z) { return pack2(tc::ex2_approx(lo2(z)), tc::ex2_approx(hi2(z))); }
+
+// 2^z on the FMA pipe for finite z <= 8: z = n + r, n the nearest integer (taken
+// from the low bits of z + 1.5 * 2^23), 2^r by the polynomial 1 + r (c1 + ...) of
+// least relative error on [-1/2, 1/2] (1.0e-4 at degree 3, 2.8e-6 at degree 4,
+// fitted by reweighted least squares), n added to the exponent.  Below -126 the
+// result is 2^-126.
+template <int DEG>
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t z) {
+    z = pack2(fmaxf(lo2(z), -126.f), fmaxf(hi2(z), -126.f));
+    const uint64_t magic = pack2(12582912.f, 12582912.f), neg = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f);
+    const uint64_t t = add2(z, magic), r = fma2(add2(t, neg), minus, z), one = pack2(1.f, 1.f);
+    uint64_t p;
+    if (DEG == 3) {
+        p = fma2(r, pack2(0.055008933f, 0.055008933f), pack2(0.24221097f, 0.24221097f));
+        p = fma2(p, r, pack2(0.6932829f, 0.6932829f));
+    } else {
+        p = fma2(r, pack2(0.009582853f, 0.009582853f), pack2(0.055906426f, 0.055906426f));
+        p = fma2(p, r, pack2(0.24024099f, 0.24024099f));
+        p = fma2(p, r, pack2(0.69312418f, 0.69312418f));
+    }
+    p = fma2(p, r, one);
+    return pack2(__uint_as_float((uint32_t)p + ((uint32_t)t << 23)),
+                 __uint_as_float((uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23)));
+}
+
 template <typename T>
 struct Pk;
 template <>
 struct Pk<__half> {
+    static constexpr int POLY = 4, DEG = 4;   // pairs of 16 whose exponentials run on the FMA pipe
     static constexpr uint32_t fmt = 0;
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -98,6 +156,7 @@ struct Pk<__half> {
 };
 template <>
 struct Pk<__nv_bfloat16> {
+    static constexpr int POLY = 4, DEG = 3;
     static constexpr uint32_t fmt = (1u << 7) | (1u << 10);   // A and B bf16
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -105,37 +164,32 @@ struct Pk<__nv_bfloat16> {
     }
 };
 
+// The whole warp waits for phase `n` of a barrier: false when it ran out of time
+// or the CTA has been given up.
+__device__ __forceinline__ bool wait_all(unsigned long long &bar, int n, volatile int *abort, int32_t *err, int code) {
+    const uint32_t b = tc::smem_u32(&bar);
+    const bool r = tc::mbar_try_wait(b, n & 1) || tc::mbar_wait_abort(b, n & 1, abort, err, code);
+    return __all_sync(0xffffffffu, r);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
 fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                  const __grid_constant__ CUtensorMap vmap, const Args a) {
     using S = Shape<D>;
-    extern __shared__ __align__(1024) unsigned char fsm_raw[];
-    unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(fsm_raw) + 1023) & ~(uintptr_t)1023);
+    // no static shared memory in this kernel: the dynamic block starts on a
+    // 1024-byte boundary, as the swizzled tiles need (checked, there is no room to shift)
+    extern __shared__ __align__(1024) unsigned char sm[];
+    if (tc::smem_u32(sm) & 1023) {
+        if (a.err) atomicExch(a.err, PK_ALIGN);
+        return;
+    }
     unsigned char *sm_q = sm, *sm_kv = sm + 2 * S::TILE;
     Bars &fb = *reinterpret_cast<Bars *>(sm + (2 + SLOTS) * S::TILE);
     volatile int *abort = &fb.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     griddep_launch_dependents();
-    if (threadIdx.x == 0) {
-        tc::mbar_init(tc::smem_u32(&fb.q_full), 1);
-        for (int s = 0; s < SLOTS; ++s) {
-            tc::mbar_init(tc::smem_u32(&fb.full[s]), 1);
-            tc::mbar_init(tc::smem_u32(&fb.freed[s]), 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(tc::smem_u32(&fb.s_full[i]), 1);
-            tc::mbar_init(tc::smem_u32(&fb.p_full[i]), 4);
-            tc::mbar_init(tc::smem_u32(&fb.pv_done[i]), 1);
-        }
-        tc::mbar_init(tc::smem_u32(&fb.fin), 1);
-        fb.abort = 0;
-        tc::fence_barrier_init();
-        tc::prefetch_tmap(&qmap);
-        tc::prefetch_tmap(&kmap);
-        tc::prefetch_tmap(&vmap);
-    }
     griddep_wait();
 
     // ---- which tokens and keys: tokens [tok0, tok0 + ntok) of the packed
@@ -175,8 +229,31 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     }
     const bool any = ntok > 0;
     const int nb = any && kend > kbeg ? (kend - kbeg + KB - 1) / KB : 0;
+    const int ns = nb ? (kend - kbeg + SB - 1) / SB : 0;   // score blocks
     const int tiles = ntok > a.TQ ? 2 : 1;
 
+    if (threadIdx.x == 0) {
+        tc::mbar_init(tc::smem_u32(&fb.q_full), 1);
+        tc::mbar_init(tc::smem_u32(&fb.skew), 1);
+        tc::mbar_init(tc::smem_u32(&fb.tail), 1);
+        for (int s = 0; s < SLOTS; ++s) {
+            tc::mbar_init(tc::smem_u32(&fb.full[s]), 1);
+            tc::mbar_init(tc::smem_u32(&fb.freed[s]), tiles);   // each tile's issuer
+        }
+        for (int i = 0; i < 2; ++i) {
+            for (int b = 0; b < 2; ++b) {
+                tc::mbar_init(tc::smem_u32(&fb.s_full[i][b]), 1);
+                tc::mbar_init(tc::smem_u32(&fb.p_full[i][b]), 4);   // the tile's softmax warps
+                tc::mbar_init(tc::smem_u32(&fb.pv_done[i][b]), 1);
+            }
+            tc::mbar_init(tc::smem_u32(&fb.fin[i]), 1);
+        }
+        fb.abort = 0;
+        tc::fence_barrier_init();
+        tc::prefetch_tmap(&qmap);
+        tc::prefetch_tmap(&kmap);
+        tc::prefetch_tmap(&vmap);
+    }
     if (warp == 2 && nb) tc::tmem_alloc(tc::smem_u32(&fb.tmem), 512);
     tc::fence_before_sync();
     __syncthreads();
@@ -234,78 +311,96 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             }
             issued = f + 1;
         }
+        // the last block ends inside 16 keys: zero the rows of V behind its last key
+        const int nv = kend - kbeg - (nb - 1) * KB;
+        if (ok && (nv & 15) && wait_all(fb.full[(2 * nb - 1) % SLOTS], (2 * nb - 1) / SLOTS, abort, a.err, PK_KV)) {
+            unsigned char *v = sm_kv + ((2 * nb - 1) % SLOTS) * S::TILE + nv * 128;
+            const int words = (16 - (nv & 15)) * 8;
+            for (int w = lane; w < words * S::HALVES; w += 32)
+                *reinterpret_cast<uint4 *>(v + (w / words) * BOX + (w % words) * 16) = make_uint4(0, 0, 0, 0);
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.tail));
+        }
         // copies in flight must land before the CTA's shared memory is released
         if (lane == 0) {
             tc::mbar_wait(tc::smem_u32(&fb.q_full), 0, nullptr, 0);
             for (int f = issued > SLOTS ? issued - SLOTS : 0; f < issued; ++f)
                 tc::mbar_wait(tc::smem_u32(&fb.full[f % SLOTS]), (f / SLOTS) & 1, nullptr, 0);
         }
-    } else if (warp == 1 && nb) {
-        // ---------------- MMA issuer (the whole warp waits, lane 0 issues) ----------------
-        constexpr uint32_t idesc_s = tc::idesc_f16_f32(TM, KB) | Pk<T>::fmt;
+    } else if ((warp == 1 || warp == 3) && nb && (warp >> 1) < tiles) {
+        // ---------------- MMA issuer of tile i (the whole warp waits, one lane issues) ----------------
+        // A warp for each tile: issuing and committing takes as long as the products,
+        // and one tile's waits must not hold up the other's products.
+        constexpr uint32_t idesc_s = tc::idesc_f16_f32(TM, SB) | Pk<T>::fmt;
         constexpr uint32_t idesc_pv = tc::idesc_f16_f32(TM, D) | (1u << 16) | Pk<T>::fmt;   // B (V) MN-major
-        auto wait = [&](unsigned long long &b, int phase, int code) -> bool {
-            const bool r = tc::mbar_wait_abort(tc::smem_u32(&b), phase & 1, abort, a.err, code);
-            return __all_sync(0xffffffffu, r);
-        };
-        auto slot_wait = [&](int f) { return wait(fb.full[f % SLOTS], f / SLOTS, PK_KV); };
-        auto issue_s = [&](int i, int j) {
+        const int i = warp >> 1;
+        // descriptors differ only in their address field (16-byte units)
+        const uint64_t qd = tc::sdesc_k_sw128(tc::smem_u32(sm_q + i * S::TILE)), kd0 = tc::sdesc_k_sw128(tc::smem_u32(sm_kv));
+        const uint64_t vd0 = tc::sdesc_mn_sw128(tc::smem_u32(sm_kv), BOX);
+        const uint32_t tS = tmem + COL_S + i * 128, tO = tmem + COL_O + i * 128;
+        auto slot_wait = [&](int f) { return wait_all(fb.full[f % SLOTS], f / SLOTS, abort, a.err, PK_KV); };
+        // scores of keys 64 n .. 64 n + 63 into buffer n & 1
+        auto issue_s = [&](int n) {
             tc::fence_after_sync();
-            if (lane == 0) {
-                const uint32_t qa = tc::smem_u32(sm_q + i * S::TILE), ka = tc::smem_u32(sm_kv + ((2 * j) % SLOTS) * S::TILE);
+            const uint64_t kd = kd0 + (uint32_t)(((n & ~1) % SLOTS) * (S::TILE >> 4) + (n & 1) * (SB * 128 >> 4));
+            const uint32_t d = tS + (n & 1) * SB;
+            if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (uint32_t)((kk >> 2) * BOX + (kk & 3) * 32);
-                    tc::mma_ss_f16(tmem + COL_S + i * 128, tc::sdesc_k_sw128(qa + off), tc::sdesc_k_sw128(ka + off), idesc_s, kk ? 1u : 0u);
+                    const uint32_t off = (uint32_t)(((kk >> 2) * BOX + (kk & 3) * 32) >> 4);
+                    tc::mma_ss_f16(d, qd + off, kd + off, idesc_s, kk ? 1u : 0u);
                 }
-                tc::mma_commit(tc::smem_u32(&fb.s_full[i]));
-                if (i == tiles - 1) tc::mma_commit(tc::smem_u32(&fb.freed[(2 * j) % SLOTS]));
+                tc::mma_commit(tc::smem_u32(&fb.s_full[i][n & 1]));
             }
             __syncwarp();
         };
-        bool ok = wait(fb.q_full, 0, PK_Q) && slot_wait(0);
-        if (ok)
-            for (int i = 0; i < tiles; ++i) issue_s(i, 0);
-        for (int j = 0; j < nb && ok; ++j) {
-            const int fv = 2 * j + 1;
+        bool ok = wait_all(fb.q_full, 0, abort, a.err, PK_Q) && slot_wait(0);
+        // tile 1 starts when tile 0 is through its first scores, so that the one's
+        // softmax meets the other's products from the start
+        if (i) ok = ok && wait_all(fb.skew, 0, abort, a.err, PK_P);
+        if (ok) {
+            issue_s(0);
+            if (ns > 1) issue_s(1);
+            if (elect_one()) tc::mma_commit(tc::smem_u32(&fb.freed[0]));
+            __syncwarp();
+        }
+        for (int n = 0; n < ns && ok; ++n) {
+            const int b = n & 1, fk = n & ~1, fv = fk + 1;   // ring fills of the block's K and V
+            const uint64_t vd = vd0 + (uint32_t)((fv % SLOTS) * (S::TILE >> 4) + b * (SB * 128 >> 4));
+            const int nv = min(SB, kend - kbeg - n * SB), ks = (nv + 15) / 16;   // 16-key steps that hold keys
             ok = slot_wait(fv);
+            if (nv & 15) ok = ok && wait_all(fb.tail, 0, abort, a.err, PK_KV);   // the rows behind the last key are zeroed
+            ok = ok && wait_all(fb.p_full[i][b], n >> 1, abort, a.err, PK_P);
             if (!ok) break;
-            const uint32_t va = tc::smem_u32(sm_kv + (fv % SLOTS) * S::TILE);
-            const int nv = min(KB, kend - kbeg - j * KB), ks = (nv + 15) / 16;   // 16-key steps that hold keys
-            if (nv & 15) {   // zero the rows behind the last key
-                const int words = (ks * 16 - nv) * 8;
-                for (int w = lane; w < words * S::HALVES; w += 32) {
-                    const int x = w / words, y = w % words;
-                    *reinterpret_cast<uint4 *>(sm_kv + (fv % SLOTS) * S::TILE + x * BOX + nv * 128 + y * 16) = make_uint4(0, 0, 0, 0);
-                }
-                tc::fence_proxy_async_smem();
-                __syncwarp();
-            }
-            for (int i = 0; i < tiles && ok; ++i) {
-                ok = wait(fb.p_full[i], j, PK_P);
-                if (!ok) break;
-                tc::fence_after_sync();
-                if (lane == 0) {
+            tc::fence_after_sync();
+            if (elect_one()) {
+                if (ks == SB / 16) {
+#pragma unroll
+                    for (int kk = 0; kk < SB / 16; ++kk)
+                        tc::mma_ts_f16(tO, tS + b * SB + kk * 8, vd + kk * 128, idesc_pv, (n | kk) ? 1u : 0u);
+                } else {
                     for (int kk = 0; kk < ks; ++kk)
-                        tc::mma_ts_f16(tmem + COL_O + i * 128, tmem + COL_S + i * 128 + kk * 8,
-                                       tc::sdesc_mn_sw128(va + kk * 2048, BOX), idesc_pv, (j | kk) ? 1u : 0u);
-                    tc::mma_commit(tc::smem_u32(&fb.pv_done[i]));
-                    if (i == tiles - 1) tc::mma_commit(tc::smem_u32(&fb.freed[fv % SLOTS]));
+                        tc::mma_ts_f16(tO, tS + b * SB + kk * 8, vd + kk * 128, idesc_pv, (n | kk) ? 1u : 0u);
                 }
-                __syncwarp();
-                if (j + 1 < nb) {
-                    if (i == 0) ok = slot_wait(2 * j + 2);
-                    // S_i lies over P_i: the product that reads it comes first
-                    ok = ok && wait(fb.pv_done[i], j, PK_PV);
-                    if (ok) issue_s(i, j + 1);
-                }
+                tc::mma_commit(tc::smem_u32(&fb.pv_done[i][b]));
             }
+            __syncwarp();
+            if (n + 2 < ns) {
+                // the next scores of this buffer lie over P: the product that reads P comes first
+                ok = slot_wait(fk + 2) && wait_all(fb.pv_done[i][b], n >> 1, abort, a.err, PK_PV);
+                if (ok) issue_s(n + 2);
+            }
+            if (ok && b && elect_one()) {   // the block's V, and the next block's K, are no longer needed here
+                tc::mma_commit(tc::smem_u32(&fb.freed[fv % SLOTS]));
+                if (n + 2 < ns) tc::mma_commit(tc::smem_u32(&fb.freed[(fk + 2) % SLOTS]));
+            }
+            __syncwarp();
         }
         // everything issued must finish before TMEM is freed
-        if (lane == 0) {
-            tc::mma_commit(tc::smem_u32(&fb.fin));
-            tc::mbar_wait(tc::smem_u32(&fb.fin), 0, nullptr, 0);
-        }
+        if (elect_one()) tc::mma_commit(tc::smem_u32(&fb.fin[i]));
+        __syncwarp();
+        tc::mbar_wait(tc::smem_u32(&fb.fin[i]), 0, nullptr, 0);
     } else if (warp >= 4 && any) {
         // ---------------- softmax and epilogue: thread = query row ----------------
         const int i = (warp - 4) >> 2, quarter = warp & 3;
@@ -325,49 +420,36 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             float m_used = -INFINITY, l = 0.f;
             bool ok = true;
             const uint32_t tS = tmem + lane_base + COL_S + i * 128, tO = tmem + lane_base + COL_O + i * 128;
-            for (int j = 0; j < nb; ++j) {
-                ok = tc::mbar_wait_abort(tc::smem_u32(&fb.s_full[i]), j & 1, abort, a.err, PK_S);
-                ok = __all_sync(0xffffffffu, ok);
+            const uint64_t sc2 = pack2(a.scale_log2, a.scale_log2);
+            for (int n = 0; n < ns; ++n) {
+                const int b = n & 1;
+                ok = wait_all(fb.s_full[i][b], n >> 1, abort, a.err, PK_S);
                 if (!ok) break;
                 tc::fence_after_sync();
-                uint32_t v[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + c * 32, v + c * 32);
+                uint32_t v[SB];
+                tc::tmem_ld32(tS + b * SB, v);
+                tc::tmem_ld32(tS + b * SB + 32, v + 32);
                 tc::tmem_wait_ld();
-                const int rel = lim - j * KB;   // columns 0..rel are seen
-                if (!__all_sync(0xffffffffu, rel >= KB - 1)) {
+                const int rel = lim - n * SB;   // columns 0..rel are seen
+                const bool full = __all_sync(0xffffffffu, rel >= SB - 1);
+                if (!full) {
 #pragma unroll
-                    for (int c = 0; c < KB; ++c)
-                        if (c > rel) v[c] = 0xff800000u;   // -inf
+                    for (int x = 0; x < SB; ++x)
+                        if (x > rel) v[x] = 0xff800000u;   // -inf
                 }
-                float mx = -INFINITY;
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < KB; ++c) mx = fmaxf(mx, __uint_as_float(v[c]));
-                mx *= a.scale_log2;
+                for (int x = 0; x < SB; x += 2)
+                    mx4[(x >> 1) & 3] = max3_nan(mx4[(x >> 1) & 3], __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
+                const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * a.scale_log2;
                 float alpha = 1.f;
                 if (mx > m_used + 8.f) {
                     alpha = m_used == -INFINITY ? 0.f : tc::ex2_approx(m_used - mx);
                     m_used = mx;
                 }
-                const float nm = m_used == -INFINITY ? 0.f : -m_used;
-                float sum = 0.f;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t p[16];
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const float p0 = tc::ex2_approx(fmaf(__uint_as_float(v[c * 32 + 2 * x]), a.scale_log2, nm));
-                        const float p1 = tc::ex2_approx(fmaf(__uint_as_float(v[c * 32 + 2 * x + 1]), a.scale_log2, nm));
-                        sum += p0 + p1;
-                        p[x] = Pk<T>::pack(p0, p1);
-                    }
-                    tc::tmem_st16(tS + c * 16, p);
-                }
-                l = l * alpha + sum;
                 // a row whose reference moved scales its O once the last product is in
-                if (j && __any_sync(0xffffffffu, alpha != 1.f)) {
-                    ok = tc::mbar_wait_abort(tc::smem_u32(&fb.pv_done[i]), (j - 1) & 1, abort, a.err, PK_PV);
-                    ok = __all_sync(0xffffffffu, ok);
+                if (n && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    ok = wait_all(fb.pv_done[i][b ^ 1], (n - 1) >> 1, abort, a.err, PK_PV);
                     if (!ok) break;
                     tc::fence_after_sync();
 #pragma unroll 1
@@ -380,17 +462,31 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                         tc::tmem_st16(tO + c * 16, o);
                     }
                 }
+                const float nm = m_used == -INFINITY ? 0.f : -m_used;
+                const uint64_t nm2 = pack2(nm, nm);
+                uint64_t sum2[2] = {0, 0};
+                uint32_t p[SB / 2];
+#pragma unroll
+                for (int x = 0; x < SB / 2; ++x) {
+                    const uint64_t z = fma2(pack2(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), sc2, nm2);
+                    const uint64_t e = exp2_unit(z);
+                    sum2[x & 1] = add2(sum2[x & 1], e);
+                    p[x] = Pk<T>::pack(lo2(e), hi2(e));
+                }
+                tc::tmem_st32(tS + b * SB, p);
                 tc::tmem_wait_st();
                 tc::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.p_full[i]));
+                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.p_full[i][b]));
+                if (n == 0 && warp == 4 && lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.skew));
+                sum2[0] = add2(sum2[0], sum2[1]);
+                l = l * alpha + (lo2(sum2[0]) + hi2(sum2[0]));
             }
             if (ok && nb) {
-                ok = tc::mbar_wait_abort(tc::smem_u32(&fb.pv_done[i]), (nb - 1) & 1, abort, a.err, PK_PV);
-                ok = __all_sync(0xffffffffu, ok) && !*abort;
+                ok = wait_all(fb.pv_done[i][(ns - 1) & 1], (ns - 1) >> 1, abort, a.err, PK_PV) && !*abort;
+                ok = __all_sync(0xffffffffu, ok);
                 tc::fence_after_sync();
             }
-            ok = __all_sync(0xffffffffu, ok);
             if (ok) {
                 const int gh = r - j0 * a.G;
                 const float inv = l != 0.f ? 1.f / l : 0.f;
