@@ -42,6 +42,7 @@ struct RopeAppendArgs {
     const int32_t *trow, *tpos;
     void *q_out;
     int32_t *err;
+    int sm_count;
 };
 cudaError_t rope_append(const PagedKV &kv, const mlxcat_rope &rope, const RopeAppendArgs &a, cudaStream_t st);
 

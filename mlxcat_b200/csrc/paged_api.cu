@@ -180,7 +180,7 @@ int mlxcat_op_rope_append(const mlxcat_paged_kv *c, const mlxcat_rope *rope, con
     } in[3] = {{q, q_stride, n_heads}, {k, k_stride, kv.n_kv}, {v, v_stride, kv.n_kv}};
     for (const auto &x : in) {
         if (!x.p) continue;
-        if (!aligned16(x.p) || x.stride % 8 || x.stride < x.heads * kv.D || x.stride > ((int64_t)1 << 38))
+        if (!aligned16(x.p) || x.stride % 8 || x.stride < x.heads * kv.D || x.stride > ((int64_t)1 << 30))
             return op_error(MLXCAT_E_INVALID, "rope append: inputs must be 16-byte aligned, token strides multiples of 8 that hold their heads");
         if (q_out) {
             const char *a0 = static_cast<const char *>(x.p), *a1 = a0 + ((M - 1) * x.stride + x.heads * kv.D) * es;
@@ -195,6 +195,8 @@ int mlxcat_op_rope_append(const mlxcat_paged_kv *c, const mlxcat_rope *rope, con
     a.in_dtype = in_dtype; a.M = M; a.n_heads = n_heads; a.with_rope = rope ? 1 : 0;
     a.q_norm = q_norm; a.k_norm = k_norm; a.eps = eps;
     a.trow = trow; a.tpos = tpos; a.q_out = q_out; a.err = err;
+    a.sm_count = sm_count();
+    if (a.sm_count <= 0) return op_error(MLXCAT_E_CUDA, "rope append: no CUDA device");
     const mlxcat_rope none = {};
     const cudaError_t e = rope_append(kv, rope ? *rope : none, a, (cudaStream_t)stream);
     if (e != cudaSuccess) return op_error(MLXCAT_E_CUDA, "rope append: %s", cudaGetErrorString(e));

@@ -14,6 +14,8 @@
 // token: its r/2 angles are computed once for all its heads.  A thread owns 8
 // consecutive features (16-byte stores); a head is D/8 neighbouring lanes, so
 // the sum of squares and the rotation partner of the half layout are shuffles.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
@@ -23,6 +25,9 @@ namespace mlxcat {
 namespace {
 
 constexpr int RA_THREADS = 256;
+constexpr int RA_BATCH = 2;   // rounds of heads whose loads are in flight together
+template <typename TI>
+constexpr int ra_ctas() { return sizeof(TI) == 4 ? 2 : 3; }   // per SM: fp32 inputs take twice the registers
 
 template <typename T>
 __device__ __forceinline__ float to_f(T x);
@@ -33,133 +38,279 @@ __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x)
 template <>
 __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 
+// two values rounded into one 32-bit word
 template <typename T>
-__device__ __forceinline__ T from_f(float x);
+__device__ __forceinline__ uint32_t from_2f(float a, float b);
 template <>
-__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+__device__ __forceinline__ uint32_t from_2f<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
 template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ uint32_t from_2f<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
 
+// Two fp32 values in one register pair: products and sums of both in one
+// instruction (the kernel is bound by its instruction rate before it is by HBM).
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// 8 consecutive elements as they lie in memory, converted when they are used
 template <typename TI>
-__device__ __forceinline__ void load8(const TI *p, float *x) {
-    constexpr int W = sizeof(TI) / 2;   // 16-byte words per 8 elements
-    __align__(16) TI v[8];
+struct Vec8 {
+    static constexpr int W = sizeof(TI) / 2;   // 16-byte words
+    uint4 w[W];
+    __device__ __forceinline__ void load(const TI *p) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) reinterpret_cast<uint4 *>(v)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        for (int i = 0; i < W; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    }
+    __device__ __forceinline__ void get(uint64_t *x) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f<TI>(v[i]);
+        for (int i = 0; i < 4; ++i)
+            x[i] = two(to_f<TI>(reinterpret_cast<const TI *>(w)[2 * i]), to_f<TI>(reinterpret_cast<const TI *>(w)[2 * i + 1]));
+    }
+};
+
+// Where the partner of a feature's pair is.  A thread holds features d0..d0+7
+// and D/2 + d0..+7 of a head.  OWN: next to it (interleaved layout, or no
+// rotation); HALF: at the same place of the thread's other 8 (half layout, whole
+// head); LANE: at the same place of another lane's first 8 (half layout, at most
+// half the head, half the rotary width a multiple of 8); ANY: read again.
+enum Partner { OWN, HALF, LANE, ANY };
+
+template <typename TI, typename TO, int D, int PARTNER>
+__global__ void __launch_bounds__(RA_THREADS, ra_ctas<TI>())
+rope_append_kernel(const PagedKV kv, const __grid_constant__ mlxcat_rope rope, const RopeAppendArgs a, int chunks, int per) {
+    constexpr int LPH = D / 16, HPI = 32 / LPH;   // lanes per head, heads of a warp at a time
+    __shared__ __align__(16) float cosv[RA_THREADS / 32][D / 2], sinv[RA_THREADS / 32][D / 2];
+    __shared__ __align__(16) float nw[2][D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int nq = a.q ? a.n_heads : 0, heads = nq + 2 * kv.n_kv;
+    const int j = lane % LPH, d0 = j * 8, hl0 = lane / LPH;
+    const int half = a.with_rope ? rope.rotary_dim / 2 : 0;
+    const bool norms = a.q_norm || a.k_norm;
+    float *cw = cosv[warp], *sw = sinv[warp];
+    griddep_launch_dependents();
+    griddep_wait();
+    if (norms) {
+        for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+            const float *w = i < D ? a.q_norm : a.k_norm;
+            if (w) nw[i / D][i % D] = __ldg(w + i % D);
+        }
+        __syncthreads();
+    }
+    // a unit: `per` rounds of HPI heads of one token; a warp takes every n-th unit
+    const int units = a.M * chunks, nwarps = gridDim.x * (RA_THREADS / 32);
+    int u = blockIdx.x * (RA_THREADS / 32) + warp;
+    if (u >= units) return;
+    auto fetch = [&](int m, int h0, int round, Vec8<TI> (*in)[2]) {
+        const int hb = h0 + round * HPI + hl0;
+#pragma unroll
+        for (int b = 0; b < RA_BATCH; ++b) {
+            const int hh = hb + b * HPI;
+            if (round + b < per && hh < heads) {
+                const bool is_q = hh < nq, is_v = hh >= nq + kv.n_kv;
+                const TI *p = reinterpret_cast<const TI *>(is_q ? a.q : is_v ? a.v : a.k) +
+                              (int64_t)m * (int)(is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) +
+                              (is_q ? hh : is_v ? hh - nq - kv.n_kv : hh - nq) * D + d0;
+                in[b][0].load(p);
+                in[b][1].load(p + D / 2);
+            }
+        }
+    };
+    Vec8<TI> cur[RA_BATCH][2], nxt[RA_BATCH][2];
+    int m = u / chunks, h0 = (u - m * chunks) * per * HPI, mn = m, hn = h0;   // of this unit and the next
+    fetch(m, h0, 0, cur);
+    int row = __ldg(a.trow + m), pos = __ldg(a.tpos + m);
+    for (; u < units; u += nwarps, m = mn, h0 = hn) {
+        // the token's slot; one outside the table or the cache is not written
+        int bad = 0, page = 0;
+        if (row >= kv.rows) bad = PE_ROW;
+        else if (pos < 0 || pos >= paged_capacity(kv)) bad = PE_POS;
+        else if (row >= 0) {
+            page = __ldg(kv.table + (size_t)row * kv.max_pages + (pos >> kv.page_shift));
+            if (page < 0 || page >= kv.n_pages) bad = PE_PAGE;
+        }
+        const int64_t at = bad ? -1 : (int64_t)page * kv.page_stride + (int64_t)(pos & ((1 << kv.page_shift) - 1)) * kv.token_stride;
+        const bool on = row >= 0;   // else padding
+        if (on && bad && lane == 0 && a.err) atomicExch(a.err, bad);
+        // angles
+        __syncwarp();
+        for (int i = lane; i < half; i += 32) {
+            const double x = (double)pos * rope.turns[i];
+            float s, c;
+            sincospif(2.0f * (float)(x - rint(x)), &s, &c);
+            cw[i] = c * rope.mscale;
+            sw[i] = s * rope.mscale;
+        }
+        __syncwarp();
+        // what this lane's features turn by in every head (HALF: pairs d0..d0+7; OWN: d0/2..+3 and D/4 + d0/2..+3)
+        float cs[8], sn[8];
+        if (half && (PARTNER == HALF || PARTNER == OWN)) {
+            const int p0 = PARTNER == HALF ? d0 : d0 / 2, p1 = PARTNER == HALF ? d0 + 4 : D / 4 + d0 / 2;
+            *reinterpret_cast<float4 *>(cs) = *reinterpret_cast<const float4 *>(cw + p0);
+            *reinterpret_cast<float4 *>(cs + 4) = *reinterpret_cast<const float4 *>(cw + p1);
+            *reinterpret_cast<float4 *>(sn) = *reinterpret_cast<const float4 *>(sw + p0);
+            *reinterpret_cast<float4 *>(sn + 4) = *reinterpret_cast<const float4 *>(sw + p1);
+        }
+        if (u + nwarps < units) {
+            mn = (u + nwarps) / chunks;
+            hn = (u + nwarps - mn * chunks) * per * HPI;
+            row = __ldg(a.trow + mn);
+            pos = __ldg(a.tpos + mn);
+        }
+#pragma unroll 1
+        for (int round = 0; round < per; round += RA_BATCH) {
+            if (round + RA_BATCH < per) fetch(m, h0, round + RA_BATCH, nxt);
+            else if (u + nwarps < units) fetch(mn, hn, 0, nxt);
+#pragma unroll
+            for (int b = 0; b < RA_BATCH; ++b) {
+                const int hb = h0 + (round + b) * HPI, hh = hb + hl0;
+                if (!on || round + b >= per || hb >= heads) break;   // uniform: every lane shuffles
+                const bool in = hh < heads, is_q = hh < nq, is_v = hh >= nq + kv.n_kv;
+                uint64_t x[2][4];
+                cur[b][0].get(x[0]);
+                cur[b][1].get(x[1]);
+                const bool norm = is_q ? a.q_norm != nullptr : !is_v && a.k_norm != nullptr;
+                const float *w = nw[is_q ? 0 : 1];
+                float r = 1.f;
+                if (norms) {
+                    uint64_t s2 = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s2 = fma2(x[i >> 2][i & 3], x[i >> 2][i & 3], s2);
+                    float ss = lo(s2) + hi(s2);
+#pragma unroll
+                    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    if (norm) {
+                        r = rsqrtf(ss * (1.0f / D) + a.eps);
+                        const uint64_t r2 = two(r, r);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float4 w4 = *reinterpret_cast<const float4 *>(w + (i >> 1) * (D / 2) + d0 + (i & 1) * 4);
+                            uint64_t *y = &x[i >> 1][(i & 1) * 2];
+                            y[0] = mul2(mul2(y[0], r2), two(w4.x, w4.y));
+                            y[1] = mul2(mul2(y[1], r2), two(w4.z, w4.w));
+                        }
+                    }
+                }
+                const bool turn = half && !is_v;
+                if (PARTNER == HALF) {
+                    if (turn) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint64_t c2 = two(cs[2 * i], cs[2 * i + 1]), s2 = two(sn[2 * i], sn[2 * i + 1]);
+                            const uint64_t e = x[0][i], f = x[1][i], fs = mul2(f, s2);
+                            x[0][i] = fma2(e, c2, two(-lo(fs), -hi(fs)));
+                            x[1][i] = fma2(f, c2, mul2(e, s2));
+                        }
+                    }
+                } else if (PARTNER == OWN) {
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const int n = half - (v * (D / 2) + d0) / 2;   // pairs of this 8 that turn
+                        if (turn && n >= 4) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float e = lo(x[v][i]), f = hi(x[v][i]);
+                                x[v][i] = two(e * cs[v * 4 + i] - f * sn[v * 4 + i], f * cs[v * 4 + i] + e * sn[v * 4 + i]);
+                            }
+                        } else if (turn && n > 0) {
+#pragma unroll
+                            for (int i = 0; i < 3; ++i) {
+                                const float e = lo(x[v][i]), f = hi(x[v][i]);
+                                if (i < n) x[v][i] = two(e * cs[v * 4 + i] - f * sn[v * 4 + i], f * cs[v * 4 + i] + e * sn[v * 4 + i]);
+                            }
+                        }
+                    }
+                } else if (PARTNER == LANE) {
+                    const int hv = half >> 3, from = lane + (j < 2 * hv ? (j < hv ? hv : -hv) : 0);
+                    const int p = j < hv ? d0 : d0 - half;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint64_t y = __shfl_sync(0xffffffffu, x[0][i], from);
+                        if (turn && j < 2 * hv) {
+                            const float2 c2 = *reinterpret_cast<const float2 *>(cw + p + 2 * i), s2 = *reinterpret_cast<const float2 *>(sw + p + 2 * i);
+                            x[0][i] = fma2(y, j < hv ? two(-s2.x, -s2.y) : two(s2.x, s2.y), mul2(x[0][i], two(c2.x, c2.y)));
+                        }
+                    }
+                } else if (turn && in) {
+                    const TI *head = reinterpret_cast<const TI *>(is_q ? a.q : a.k) + (int64_t)m * (int)(is_q ? a.q_stride : a.k_stride) +
+                                     (is_q ? hh : hh - nq) * D;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int d = (i >> 3) * (D / 2) + d0 + (i & 7), e = d < half ? d + half : d - half;
+                        if (d >= 2 * half) continue;
+                        float y = to_f<TI>(head[e]);
+                        if (norm) y = y * r * w[e];
+                        const int p = d < half ? d : e;
+                        const uint64_t o = x[i >> 3][(i & 7) >> 1];
+                        const float z = (i & 1) ? hi(o) : lo(o), v = d < half ? z * cw[p] - y * sw[p] : z * cw[p] + y * sw[p];
+                        x[i >> 3][(i & 7) >> 1] = (i & 1) ? two(lo(o), v) : two(v, hi(o));
+                    }
+                }
+                if (in && (is_q || at >= 0)) {
+                    TO *to = is_q ? reinterpret_cast<TO *>(a.q_out) + ((int64_t)m * a.n_heads + hh) * D + d0
+                                  : reinterpret_cast<TO *>(is_v ? kv.v : kv.k) + at + (int64_t)(is_v ? hh - nq - kv.n_kv : hh - nq) * kv.head_stride + d0;
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        uint4 out;
+                        out.x = from_2f<TO>(lo(x[v][0]), hi(x[v][0]));
+                        out.y = from_2f<TO>(lo(x[v][1]), hi(x[v][1]));
+                        out.z = from_2f<TO>(lo(x[v][2]), hi(x[v][2]));
+                        out.w = from_2f<TO>(lo(x[v][3]), hi(x[v][3]));
+                        *reinterpret_cast<uint4 *>(to + v * (D / 2)) = out;
+                    }
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < RA_BATCH; ++b) { cur[b][0] = nxt[b][0]; cur[b][1] = nxt[b][1]; }
+        }
+    }
+}
+
+template <typename TI, typename TO, int D, int PARTNER>
+cudaError_t launch_t(const PagedKV &kv, const mlxcat_rope &rope, const RopeAppendArgs &a, cudaStream_t st) {
+    constexpr int HPI = 32 / (D / 16), WARPS = RA_THREADS / 32;
+    const int rounds = ((a.q ? a.n_heads : 0) + 2 * kv.n_kv + HPI - 1) / HPI;
+    const int64_t wave = (int64_t)ra_ctas<TI>() * a.sm_count * WARPS;
+    // few tokens: their heads are spread over the warps of a wave; many: a warp
+    // takes a token's heads one after the other and forms its angles once
+    const int spread = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, wave / a.M));
+    const int per = (rounds + spread - 1) / spread, chunks = (rounds + per - 1) / per;
+    const int64_t units = (int64_t)a.M * chunks;
+    if (units > 0x3fffffff) return cudaErrorInvalidValue;
+    const unsigned grid = (unsigned)std::min<int64_t>((units + WARPS - 1) / WARPS, wave / WARPS);
+    return launch_pdl(rope_append_kernel<TI, TO, D, PARTNER>, dim3(grid), dim3(RA_THREADS), 0, st, kv, rope, a, chunks, per);
 }
 
 template <typename TI, typename TO, int D>
-__global__ void __launch_bounds__(RA_THREADS)
-rope_append_kernel(const PagedKV kv, const __grid_constant__ mlxcat_rope rope, const RopeAppendArgs a) {
-    constexpr int LPH = D / 8;   // lanes per head
-    __shared__ float2 cs[D / 2];
-    griddep_launch_dependents();
-    griddep_wait();
-    const int m = blockIdx.x;
-    const int row = __ldg(a.trow + m), pos = __ldg(a.tpos + m);
-    if (row < 0) return;   // padding
-    const int half = a.with_rope ? rope.rotary_dim / 2 : 0;
-    for (int i = threadIdx.x; i < half; i += RA_THREADS) {
-        const double turns = (double)pos * rope.turns[i];
-        float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        cs[i] = make_float2(c * rope.mscale, s * rope.mscale);
-    }
-    // the token's slot; one outside the table or the cache is not written
-    int page = -1;
-    int bad = 0;
-    if (row >= kv.rows) bad = PE_ROW;
-    else if (pos < 0 || pos >= paged_capacity(kv)) bad = PE_POS;
-    else {
-        page = __ldg(kv.table + (size_t)row * kv.max_pages + (pos >> kv.page_shift));
-        if (page < 0 || page >= kv.n_pages) { bad = PE_PAGE; page = -1; }
-    }
-    if (bad && threadIdx.x == 0 && a.err) atomicExch(a.err, bad);
-    const int64_t slot = page < 0 ? 0 : (int64_t)page * kv.page_stride +
-                                            (int64_t)(pos & ((1 << kv.page_shift) - 1)) * kv.token_stride;
-    __syncthreads();
-    const int nq = a.q ? a.n_heads : 0, heads = nq + 2 * kv.n_kv;
-    const int vecs = heads * LPH;
-    const bool inter = rope.layout == MLXCAT_ROPE_INTERLEAVED;
-    for (int v0 = threadIdx.x & ~31; v0 < vecs; v0 += RA_THREADS) {   // warp-uniform bound: every lane shuffles
-        const int vi = v0 + (threadIdx.x & 31);
-        const bool on = vi < vecs;
-        const int hh = (on ? vi : vecs - 1) / LPH, j = (on ? vi : vecs - 1) % LPH, d0 = j * 8;
-        const bool is_q = hh < nq, is_v = hh >= nq + kv.n_kv;
-        const int hl = is_q ? hh : is_v ? hh - nq - kv.n_kv : hh - nq;
-        const TI *src = reinterpret_cast<const TI *>(is_q ? a.q : is_v ? a.v : a.k) +
-                        (int64_t)m * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) + (int64_t)hl * D;
-        float x[8];
-        load8<TI>(src + d0, x);
-        const float *w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-#pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        float r = 1.f;
-        if (w) {
-            r = 1.0f / sqrtf(ss / (float)D + a.eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * r * __ldg(w + d0 + i);
-        }
-        if (half) {
-            if (inter) {
-                if (!is_v) {
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2)
-                        if (d0 + i < 2 * half) {
-                            const float2 t = cs[(d0 + i) >> 1];
-                            const float p = x[i], q = x[i + 1];
-                            x[i] = p * t.x - q * t.y;
-                            x[i + 1] = q * t.x + p * t.y;
-                        }
-                }
-            } else if ((half & 7) == 0) {
-                // partner vector: half/8 lanes on or back, same register
-                const int hv = half >> 3;
-                const bool lo = j < hv, in = j < 2 * hv;
-                const int lane = threadIdx.x & 31, from = in ? (lo ? lane + hv : lane - hv) : lane;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float o = __shfl_sync(0xffffffffu, x[i], from);
-                    if (in && !is_v) {
-                        const float2 t = cs[lo ? d0 + i : d0 + i - half];
-                        x[i] = lo ? x[i] * t.x - o * t.y : x[i] * t.x + o * t.y;
-                    }
-                }
-            } else if (!is_v) {
-                // a rotary width whose half is no multiple of 8: the partner is read again
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int d = d0 + i;
-                    if (d >= 2 * half) continue;
-                    const int e = d < half ? d + half : d - half;
-                    float o = to_f<TI>(src[e]);
-                    if (w) o = o * r * __ldg(w + e);
-                    const float2 t = cs[d < half ? d : e];
-                    x[i] = d < half ? x[i] * t.x - o * t.y : x[i] * t.x + o * t.y;
-                }
-            }
-        }
-        if (!on) continue;
-        __align__(16) TO y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = from_f<TO>(x[i]);
-        TO *dst = nullptr;
-        if (is_q) dst = reinterpret_cast<TO *>(a.q_out) + ((size_t)m * a.n_heads + hl) * D;
-        else if (page >= 0) dst = reinterpret_cast<TO *>(is_v ? kv.v : kv.k) + slot + (int64_t)hl * kv.head_stride;
-        if (dst) *reinterpret_cast<uint4 *>(dst + d0) = *reinterpret_cast<const uint4 *>(y);
-    }
+cudaError_t launch_p(const PagedKV &kv, const mlxcat_rope &rope, const RopeAppendArgs &a, cudaStream_t st) {
+    if (!a.with_rope || rope.layout == MLXCAT_ROPE_INTERLEAVED) return launch_t<TI, TO, D, OWN>(kv, rope, a, st);
+    if (rope.rotary_dim == D) return launch_t<TI, TO, D, HALF>(kv, rope, a, st);
+    if (rope.rotary_dim % 16 || rope.rotary_dim > D / 2) return launch_t<TI, TO, D, ANY>(kv, rope, a, st);
+    return launch_t<TI, TO, D, LANE>(kv, rope, a, st);
 }
 
 template <typename TI, typename TO>
 cudaError_t launch_d(const PagedKV &kv, const mlxcat_rope &rope, const RopeAppendArgs &a, cudaStream_t st) {
-    if (kv.D == 128)
-        return launch_pdl(rope_append_kernel<TI, TO, 128>, dim3(a.M), dim3(RA_THREADS), 0, st, kv, rope, a);
-    return launch_pdl(rope_append_kernel<TI, TO, 64>, dim3(a.M), dim3(RA_THREADS), 0, st, kv, rope, a);
+    return kv.D == 128 ? launch_p<TI, TO, 128>(kv, rope, a, st) : launch_p<TI, TO, 64>(kv, rope, a, st);
 }
 
 template <typename TI>
