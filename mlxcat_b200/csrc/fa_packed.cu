@@ -143,6 +143,13 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t z) {
                  __uint_as_float((uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23)));
 }
 
+// a whole 32-byte sector per thread: rows lie apart, so 16-byte stores would fill
+// every sector twice
+__device__ __forceinline__ void store32(void *p, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
 template <typename T>
 struct Pk;
 template <>
@@ -189,8 +196,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     volatile int *abort = &fb.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    griddep_launch_dependents();
+    // the kernel that follows a prefix pass starts on the SMs that this one leaves
+    // free, without waiting for it: so the pass's own predecessor must be done first
     griddep_wait();
+    griddep_launch_dependents();
 
     // ---- which tokens and keys: tokens [tok0, tok0 + ntok) of the packed
     // queries, keys [kbeg, kend) counted from the sequence's start
@@ -490,6 +499,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             if (ok) {
                 const int gh = r - j0 * a.G;
                 const float inv = l != 0.f ? 1.f / l : 0.f;
+                const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
                 T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(tok0 + tk) * a.Hq + h * a.G + gh) * D;
                 const size_t prow = ((size_t)split * a.Hkv + h) * ((size_t)a.M * a.G) + (size_t)(tok0 + tk) * a.G + gh;
 #pragma unroll 1
@@ -505,17 +515,22 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     for (int x = 0; x < 32; ++x)
                         if (!live) acc[x] = 0u;
                     if (!pad && a.prefix) {
-                        uint4 *p = reinterpret_cast<uint4 *>(a.o_part + prow * D + c * 32);
+                        float *p = a.o_part + prow * D + c * 32;
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) p[x] = make_uint4(acc[4 * x], acc[4 * x + 1], acc[4 * x + 2], acc[4 * x + 3]);
+                        for (int x = 0; x < 4; ++x) store32(p + x * 8, acc + x * 8);
                     } else if (!pad) {
                         uint32_t y[16];
 #pragma unroll
                         for (int x = 0; x < 16; ++x)
                             y[x] = Pk<T>::pack(__uint_as_float(acc[2 * x]) * inv, __uint_as_float(acc[2 * x + 1]) * inv);
+                        if (wide) {
+                            store32(dst + c * 32, y);
+                            store32(dst + c * 32 + 16, y + 8);
+                        } else {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            reinterpret_cast<uint4 *>(dst + c * 32)[x] = make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
+                            for (int x = 0; x < 4; ++x)
+                                reinterpret_cast<uint4 *>(dst + c * 32)[x] = make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
+                        }
                     }
                 }
                 if (a.prefix && !pad) *reinterpret_cast<float2 *>(a.ml_part + prow * 2) = make_float2(m_used, l);

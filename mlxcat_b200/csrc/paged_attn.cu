@@ -39,6 +39,10 @@ constexpr int TK = 16;             // keys per warp tile
 constexpr int UNIT = PW * TK;      // keys per unit
 constexpr int ST = 3;              // ring stages per warp
 constexpr int CTAS_PER_SM = 2;
+// An item costs a CTA about as much to begin and end (queries, page lookups, first
+// loads, merge: 5,500 cycles) as three units of keys: its stretch has that many
+// units without keys in front, so that CTAs of many short items are not the last.
+constexpr int LEAD = 3;
 
 template <typename T>
 struct Half2;
@@ -87,33 +91,14 @@ __device__ __forceinline__ void cpa16(uint32_t s, const void *g, int bytes) {
 }
 
 // What a group of tokens sees: its row and one past its last key (clamped to
-// what the table holds).  Every lane of the warp gets the same answer.
+// what the table holds).
 struct Group {
     int row, kend;
 };
-__device__ __forceinline__ Group group_of(const PagedKV &kv, const PagedQuery &a, int grp) {
-    const int lane = threadIdx.x & 31, t0 = grp * a.qg, n = min(a.qg, a.M - t0);
-    int row = -1, kend = 0;
-    for (int j = lane; j < n; j += 32) {
-        const int r = __ldg(a.trow + t0 + j), p = __ldg(a.tpos + t0 + j);
-        if (r >= 0) {
-            row = max(row, r);
-            kend = max(kend, p == 0x7fffffff ? p : p + 1);
-        }
-    }
-    row = __reduce_max_sync(0xffffffffu, row);
-    kend = __reduce_max_sync(0xffffffffu, kend);
-    const int cap = paged_capacity(kv);
-    if (row >= kv.rows || kend > cap) {
-        if (lane == 0 && a.err) atomicExch(a.err, row >= kv.rows ? PE_ROW : PE_POS);
-        kend = row >= kv.rows ? 0 : cap;
-    }
-    return {row, kend};
-}
-// the same for one thread (the scan over groups)
-__device__ __forceinline__ int group_units(const PagedKV &kv, const PagedQuery &a, int grp, int key_begin) {
+__device__ __forceinline__ Group group_alone(const PagedKV &kv, const PagedQuery &a, int grp) {
     const int t0 = grp * a.qg, n = min(a.qg, a.M - t0);
     int row = -1, kend = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) {
         const int r = __ldg(a.trow + t0 + j), p = __ldg(a.tpos + t0 + j);
         if (r >= 0) {
@@ -121,9 +106,12 @@ __device__ __forceinline__ int group_units(const PagedKV &kv, const PagedQuery &
             kend = max(kend, p == 0x7fffffff ? p : p + 1);
         }
     }
-    if (row < 0 || row >= kv.rows) return 0;
-    kend = min(kend, paged_capacity(kv));
-    return kend > key_begin ? (int)(((int64_t)kend - key_begin + UNIT - 1) / UNIT) : 0;
+    const int cap = paged_capacity(kv);
+    if (row >= kv.rows || kend > cap) {
+        if (a.err) atomicExch(a.err, row >= kv.rows ? PE_ROW : PE_POS);
+        kend = row >= kv.rows ? 0 : cap;
+    }
+    return {row, row < 0 ? 0 : kend};
 }
 
 __device__ __forceinline__ int64_t cta_begin(int c, int64_t U, int C) { return (int64_t)c * U / C; }
@@ -135,16 +123,19 @@ __device__ __forceinline__ float weight_of(float m, float l, float mx) {
     return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : tc::ex2_approx(m - mx);
 }
 
-// One float4 more per row keeps the merge's shared-memory stores apart.
+// Shared memory: the warps' rings, the item's query rows, their limits.  The
+// merge of the warps reuses the rings.
 template <int D, int NT>
 struct PagedShape {
     static constexpr int STAGE = 2 * TK * D * 2;            // K and V of one tile, bytes
     static constexpr int RING = PW * ST * STAGE;
     static constexpr int QR = NT * 8;                       // query rows of an item
-    static constexpr int OP = D + 4;
-    static constexpr int MERGE = PW * QR * (OP + 2) * 4;
-    static constexpr int SMEM = RING > MERGE ? RING : MERGE;
+    static constexpr int MT = D / 16, MTW = MT / PW;        // m tiles of O^T, and those a warp finishes
+    static constexpr int MERGE = PW * MT * NT * 512 + PW * QR * 8;
+    static constexpr int BODY = RING > MERGE ? RING : MERGE;
+    static constexpr int SMEM = BODY + QR * D * 2 + QR * 4;
 };
+constexpr int MAX_GROUPS = 512;   // groups whose (row, last key) a CTA keeps
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(PT, CTAS_PER_SM)
@@ -154,25 +145,40 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
     constexpr int CH = D / 8;            // 16-byte chunks per key
     constexpr int RPI = 32 / CH;         // keys per load instruction of a warp
     extern __shared__ __align__(128) unsigned char psm[];
+    unsigned char *qsm = psm + S::BODY;                                       // [QR][D], chunks swizzled
+    int *lim_s = reinterpret_cast<int *>(qsm + S::QR * D * 2);                // [QR]
     __shared__ int64_t wsum[PW];
     __shared__ int64_t start_s[2];       // group of the first unit, units before it
+    __shared__ Group info[MAX_GROUPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int Hq = a.n_heads, Hkv = kv.n_kv, G = Hq / Hkv;
     const int groups = (a.M + a.qg - 1) / a.qg;
     const int qts = (a.qg * G + S::QR - 1) / S::QR;
     const int per_group = Hkv * qts;     // items of a group: (query tile, KV head)
+    const uint32_t inv_g = (uint32_t)((0x100000000ull + G - 1) / G);   // row / G by one product: row < 2^26
+    auto div_g = [&](int x) { return G == 1 ? x : (int)__umulhi((uint32_t)x, inv_g); };
+    // units of an item of the group, the leading ones among them; 0 without keys
+    auto units_of = [&](const Group &x) { return x.kend > key_begin ? (x.kend - key_begin + UNIT - 1) / UNIT + LEAD : 0; };
 
+    // Behind a prefix pass this kernel needs nothing of it: it starts on the SMs the
+    // pass leaves free (which itself lets it start only once all before the pass is
+    // done) and waits at its end, so that the join after it waits for both.
     griddep_launch_dependents();
-    griddep_wait();
+    if (!force_partial) griddep_wait();
 
     // ---- where this CTA's stretch of units starts: thread x sums the groups of
     // its chunk, a scan gives the total and the chunk that holds the start
     const int per = (groups + PT - 1) / PT;
+    const bool kept = groups <= MAX_GROUPS;
     int64_t mine = 0;
     {
         const int g0 = threadIdx.x * per, g1 = min(groups, g0 + per);
-        for (int i = g0; i < g1; ++i) mine += group_units(kv, a, i, key_begin);
+        for (int i = g0; i < g1; ++i) {
+            const Group x = group_alone(kv, a, i);
+            if (kept) info[i] = x;
+            mine += units_of(x);
+        }
     }
     int64_t incl = mine;
 #pragma unroll
@@ -182,6 +188,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
     }
     if (lane == 31) wsum[warp] = incl;
     __syncthreads();
+    auto group = [&](int i) { return kept ? info[i] : group_alone(kv, a, i); };
     int64_t before = incl - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < PW; ++w) {
@@ -196,7 +203,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         int64_t acc = before * per_group;
         int i = threadIdx.x * per;
         for (;; ++i) {
-            const int64_t n = (int64_t)group_units(kv, a, i, key_begin) * per_group;
+            const int64_t n = (int64_t)units_of(group(i)) * per_group;
             if (u0 < acc + n) break;
             acc += n;
         }
@@ -206,9 +213,8 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
     __syncthreads();
 
     // ---- groups without keys here: nothing else writes their outputs
-    for (int i = blockIdx.x; i < groups; i += gridDim.x) {
-        if (warp != 0) continue;
-        if (group_of(kv, a, i).kend > key_begin) continue;
+    for (int i = blockIdx.x * PW + warp; i < groups; i += gridDim.x * PW) {
+        if (units_of(group(i))) continue;
         for (int x = lane; x < per_group; x += 32) meta[(size_t)i * per_group + x] = make_int2(0, -1);
         if (force_partial) continue;
         const int t0 = i * a.qg, n = min(a.qg, a.M - t0);
@@ -218,58 +224,49 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             for (int x = lane; x < Hq * D / 8; x += 32) dst[x] = make_uint4(0, 0, 0, 0);
         }
     }
-    if (u1 <= u0) return;
+    if (u1 <= u0) {
+        if (force_partial) griddep_wait();
+        return;
+    }
 
     int grp = (int)start_s[0];
     int64_t ubase = start_s[1];          // units before this group
-    Group gi = group_of(kv, a, grp);
-    int gu = gi.kend > key_begin ? (gi.kend - key_begin + UNIT - 1) / UNIT : 0;   // units per item
+    Group gi = group(grp);
+    int gu = units_of(gi);               // units per item
     unsigned char *ring = psm + warp * (ST * S::STAGE);
-    const uint32_t ring_a = tc::smem_u32(ring);
+    const uint32_t ring_a = tc::smem_u32(ring), qsm_a = tc::smem_u32(qsm);
     const int ch = lane % CH, r0 = lane / CH;
 
     for (int64_t u = u0; u < u1;) {
         while (u >= ubase + (int64_t)gu * per_group) {
             ubase += (int64_t)gu * per_group;
-            gi = group_of(kv, a, ++grp);
-            gu = gi.kend > key_begin ? (gi.kend - key_begin + UNIT - 1) / UNIT : 0;
+            gi = group(++grp);
+            gu = units_of(gi);
         }
         const int x = (int)((u - ubase) / gu);                 // item of the group
         const int64_t ib = ubase + (int64_t)x * gu;            // its first unit
-        const int ua = (int)(u - ib), ub = (int)min((int64_t)gu, u1 - ib);
-        const bool whole = ua == 0 && ub == gu;
+        const int va = (int)(u - ib), vend = (int)min((int64_t)gu, u1 - ib);   // this CTA's part of it
+        u = ib + vend;
+        const int ua = max(va - LEAD, 0), ub = vend - LEAD;                       // units of keys
+        if (ub <= ua) continue;                                                 // leading units only
+        const bool whole = ua == 0 && vend == gu;
         const int h = x / qts, qt = x - h * qts;
         const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
         const int nq = min(S::QR, ntok * G - qt * S::QR);      // may be <= 0 in a last, short group
         const size_t item = (size_t)grp * per_group + x;
-        u = ib + ub;
 
-        // ---- query rows as B operands, key limits per column
-        uint32_t qf[NT][D / 16][2];
-        int lim[NT][2];
-        int lim_min = 0x7fffffff;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * 8 + g;
-            const int rr = qt * S::QR + r;
+        // ---- the item's query rows and key limits into shared memory
+        for (int w = threadIdx.x; w < S::QR * CH; w += PT) {
+            const int r = w / CH, c = w % CH, rr = qt * S::QR + r, j = div_g(rr);
             const bool ok = r < nq;
-            const T *src = reinterpret_cast<const T *>(a.q) +
-                           ((size_t)(t0 + (ok ? rr / G : 0)) * Hq + h * G + (ok ? rr % G : 0)) * D;
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-                qf[nt][ks][0] = ok ? __ldg(reinterpret_cast<const uint32_t *>(src + ks * 16 + 2 * t)) : 0u;
-                qf[nt][ks][1] = ok ? __ldg(reinterpret_cast<const uint32_t *>(src + ks * 16 + 8 + 2 * t)) : 0u;
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int c = nt * 8 + 2 * t + e, cc = qt * S::QR + c;
-                int l = 0x7fffffff;
-                if (c < nq && __ldg(a.trow + t0 + cc / G) >= 0) l = __ldg(a.tpos + t0 + cc / G);
-                lim[nt][e] = l;
-                lim_min = min(lim_min, l);
-            }
+            const T *src = reinterpret_cast<const T *>(a.q) + ((size_t)(t0 + (ok ? j : 0)) * Hq + h * G + (ok ? rr - j * G : 0)) * D + c * 8;
+            cpa16(qsm_a + (uint32_t)(r * D * 2 + ((c ^ (r & 7)) << 4)), src, ok ? 16 : 0);
         }
-        lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+        if (threadIdx.x < S::QR) {
+            const int r = threadIdx.x, m = t0 + div_g(qt * S::QR + r);
+            // rows nobody reads see everything: they need no mask
+            lim_s[r] = r < nq && __ldg(a.trow + m) >= 0 ? __ldg(a.tpos + m) : 0x7fffffff;
+        }
 
         float o[D / 16][NT][4], ls[NT][4], mr[NT][2];
 #pragma unroll
@@ -326,6 +323,23 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             if (s < steps) stage(s);
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         }
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 2) : "memory");   // the queries came with the first stage
+        __syncthreads();
+        // query rows as B operands, key limits of this lane's columns
+        uint32_t qf[NT][D / 16][2];
+        int lim[NT][2];
+        int lim_min = 0x7fffffff;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + (lane & 7);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks += 2)
+                ldm4(&qf[nt][ks][0], qsm_a + (uint32_t)(r * D * 2 + (((ks * 2 + (lane >> 3)) ^ (r & 7)) << 4)));
+            lim[nt][0] = lim_s[nt * 8 + 2 * t];
+            lim[nt][1] = lim_s[nt * 8 + 2 * t + 1];
+            lim_min = min(lim_min, min(lim[nt][0], lim[nt][1]));
+        }
+        lim_min = __reduce_min_sync(0xffffffffu, lim_min);
         for (int s = 0; s < steps; ++s) {
             __syncwarp();            // every lane has read the stage that is filled now
             if (s + ST - 1 < steps) stage(s + ST - 1);
@@ -407,58 +421,78 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             }
         }
 
-        // ---- merge the warps' partials through the ring's memory
+        // ---- merge the warps' partials through the rings' memory: every warp
+        // finishes MTW m tiles of O^T, as accumulator fragments [warp][m tile][nt][lane]
         asm volatile("cp.async.wait_group 0;\n" ::: "memory");
         __syncthreads();
-        float *om = reinterpret_cast<float *>(psm);                    // [PW][QR][OP]
-        float *mm = om + PW * S::QR * S::OP;                           // [PW][QR] max, then sums
-        float *lm = mm + PW * S::QR;
+        float4 *of = reinterpret_cast<float4 *>(psm);
+        float2 *mls = reinterpret_cast<float2 *>(psm + PW * S::MT * NT * 512);   // [warp][QR] (max, sum)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int c = nt * 8 + 2 * t + e;
-                float *dst = om + (warp * S::QR + c) * S::OP + g;
-#pragma unroll
-                for (int mt = 0; mt < D / 16; ++mt) {
-                    dst[mt * 16] = o[mt][nt][e];
-                    dst[mt * 16 + 8] = o[mt][nt][2 + e];
-                }
-                if (g == 0) {
-                    mm[warp * S::QR + c] = mr[nt][e];
-                    lm[warp * S::QR + c] = ls[nt][e];
-                }
+            for (int mt = 0; mt < S::MT; ++mt)
+                if (mt / S::MTW != warp)
+                    of[((warp * S::MT + mt) * NT + nt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
+            if (g == 0) {
+                mls[warp * S::QR + nt * 8 + 2 * t] = make_float2(mr[nt][0], ls[nt][0]);
+                mls[warp * S::QR + nt * 8 + 2 * t + 1] = make_float2(mr[nt][1], ls[nt][1]);
             }
+        }
         __syncthreads();
         const bool direct = whole && !force_partial;
         // slots in order of (item, CTA): unique, since a piece starts a new item or a new CTA
         const size_t slot = item + blockIdx.x;
-        for (int w = threadIdx.x; w < nq * (D / 4); w += PT) {
-            const int r = w / (D / 4), d = (w % (D / 4)) * 4;
-            float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < PW; ++i) mx = fmaxf(mx, mm[i * S::QR + r]);
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float l = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+            float f[2][PW], l[2], mx[2];
 #pragma unroll
-            for (int i = 0; i < PW; ++i) {
-                const float mi = mm[i * S::QR + r];
-                const float f = weight_of(mi, lm[i * S::QR + r], mx);
-                const float4 y = *reinterpret_cast<const float4 *>(om + (i * S::QR + r) * S::OP + d);
-                l += f * lm[i * S::QR + r];
-                acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
+            for (int e = 0; e < 2; ++e) {
+                float2 ml[PW];
+                mx[e] = -INFINITY;
+                l[e] = 0.f;
+#pragma unroll
+                for (int i = 0; i < PW; ++i) {
+                    ml[i] = mls[i * S::QR + nt * 8 + 2 * t + e];
+                    mx[e] = fmaxf(mx[e], ml[i].x);
+                }
+#pragma unroll
+                for (int i = 0; i < PW; ++i) {
+                    f[e][i] = weight_of(ml[i].x, ml[i].y, mx[e]);
+                    l[e] += f[e][i] * ml[i].y;
+                }
             }
-            if (direct) {
-                const int rr = qt * S::QR + r, m = t0 + rr / G;
-                if (__ldg(a.trow + m) < 0) continue;
-                const float inv = l != 0.f ? 1.f / l : 0.f;
-                uint2 y;
-                y.x = Half2<T>::pack(acc.x * inv, acc.y * inv);
-                y.y = Half2<T>::pack(acc.z * inv, acc.w * inv);
-                *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr % G) * D + d) = y;
-            } else {
-                *reinterpret_cast<float4 *>(o_part + (slot * S::QR + r) * D + d) = acc;
-                if (d == 0) *reinterpret_cast<float2 *>(ml_part + (slot * S::QR + r) * 2) = make_float2(mx, l);
+            const int ra = nt * 8 + 2 * t;                       // this lane's two query rows
+            if (!direct && warp == 0 && g == 0) {
+                if (ra < nq) *reinterpret_cast<float2 *>(ml_part + (slot * S::QR + ra) * 2) = make_float2(mx[0], l[0]);
+                if (ra + 1 < nq) *reinterpret_cast<float2 *>(ml_part + (slot * S::QR + ra + 1) * 2) = make_float2(mx[1], l[1]);
+            }
+            const float inv0 = l[0] != 0.f ? 1.f / l[0] : 0.f, inv1 = l[1] != 0.f ? 1.f / l[1] : 0.f;
+            // 16-bit results go out as pairs of features: even g the first row's, odd g the second's
+            const int rw = ra + (g & 1), rr = qt * S::QR + rw, j = div_g(rr), m = t0 + j;
+            const bool write = rw < nq && (!direct || __ldg(a.trow + m) >= 0);
+            T *dst = reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr - j * G) * D + (g & ~1);
+#pragma unroll
+            for (int mt = 0; mt < S::MT; ++mt) {
+                if (mt / S::MTW != warp) continue;
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < PW; ++i) {
+                    const float4 z = i == warp ? make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3])
+                                               : of[((i * S::MT + mt) * NT + nt) * 32 + lane];
+                    y[0] += f[0][i] * z.x; y[1] += f[1][i] * z.y; y[2] += f[0][i] * z.z; y[3] += f[1][i] * z.w;
+                }
+                if (direct) {
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        const float v0 = y[2 * hh] * inv0, v1 = y[2 * hh + 1] * inv1;
+                        const float z = __shfl_xor_sync(0xffffffffu, (g & 1) ? v0 : v1, 4);
+                        if (write) *reinterpret_cast<uint32_t *>(dst + mt * 16 + hh * 8) = (g & 1) ? Half2<T>::pack(z, v1) : Half2<T>::pack(v0, z);
+                    }
+                } else {
+                    float *dp = o_part + (slot * S::QR + ra) * D + mt * 16 + g;
+                    if (ra < nq) { dp[0] = y[0]; dp[8] = y[2]; }
+                    if (ra + 1 < nq) { dp[D] = y[1]; dp[D + 8] = y[3]; }
+                }
             }
         }
         // the CTA that holds an item's first unit says where its pieces are
@@ -468,6 +502,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         }
         __syncthreads();   // the ring is filled again
     }
+    if (force_partial) griddep_wait();
 }
 
 // Merge an item's pieces (and, after a shared prefix, the prefix's splits):
@@ -487,7 +522,7 @@ attn_join(const PagedKV kv, const PagedQuery a, int QR, const float *__restrict_
     const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
     const int nq = min(QR, ntok * G - qt * QR);
     const int n_own = mt.y >= 0 ? mt.y - mt.x + 1 : 0, n = n_own + pre.splits;
-    constexpr int PB = 4;   // pieces whose loads are in flight together
+    constexpr int PB = 6;   // pieces whose loads are in flight together
     for (int w = threadIdx.x; w < nq * (D / 8); w += blockDim.x) {
         const int r = w / (D / 8), d = (w % (D / 8)) * 8;
         const int rr = qt * QR + r, m = t0 + rr / G;
