@@ -23,8 +23,9 @@
 // are zeroed in shared memory before the product, so what lies behind a
 // sequence (another prompt, an unwritten page, NaN) does not reach it.
 //
-// Warps: 0 TMA producer, 1 and 3 MMA issuers of tiles 0 and 1, 2 TMEM
-// allocation, 4-7 softmax of tile 0, 8-11 of tile 1.  Every wait is bounded; a timeout sets *err and an abort
+// Warps: 0 TMEM allocation and TMA producer, 1 and 2 issuers of the products with
+// V of tiles 0 and 1, 3 and 12 issuers of their scores, 4-7 softmax of tile 0,
+// 8-11 of tile 1.  Every wait is bounded; a timeout sets *err and an abort
 // flag after which every role skips its work, the producer waits for its copies
 // and the issuer for what it committed, and the CTA frees TMEM.
 #include <cuda.h>
@@ -46,15 +47,15 @@ namespace {
 constexpr int TM = 128;                 // query rows of a tile (MMA M)
 constexpr int KB = 128;                 // keys of a block
 constexpr int BOX = 128 * 128;          // [128 rows][64 features] swizzled
-constexpr int SLOTS = 5;                // K / V ring
-constexpr int THREADS = 384;
+constexpr int KSLOTS = 2, VSLOTS = 3;   // rings of K and V blocks
+constexpr int THREADS = 416;
 constexpr int SB = 64;                  // keys of a score buffer: two per tile
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
 enum PkErr { PK_Q = 61, PK_KV, PK_FREE, PK_S, PK_P, PK_PV, PK_ALIGN };
 
 struct Bars {
-    unsigned long long q_full, full[SLOTS], freed[SLOTS], skew, tail, fin[2];
+    unsigned long long q_full, k_full[KSLOTS], k_free[KSLOTS], v_full[VSLOTS], v_free[VSLOTS], skew, tail, fin[4];
     unsigned long long s_full[2][2], p_full[2][2], pv_done[2][2];   // [tile][score buffer]
     uint32_t tmem;
     int abort;
@@ -64,7 +65,7 @@ template <int D>
 struct Shape {
     static constexpr int HALVES = D / 64;
     static constexpr int TILE = HALVES * BOX;
-    static constexpr int SMEM = (2 + SLOTS) * TILE + (int)sizeof(Bars);
+    static constexpr int SMEM = (2 + KSLOTS + VSLOTS) * TILE + (int)sizeof(Bars);
     static_assert(SMEM <= 227 * 1024, "two Q tiles and the ring must fit one CTA");
 };
 
@@ -191,8 +192,8 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         if (a.err) atomicExch(a.err, PK_ALIGN);
         return;
     }
-    unsigned char *sm_q = sm, *sm_kv = sm + 2 * S::TILE;
-    Bars &fb = *reinterpret_cast<Bars *>(sm + (2 + SLOTS) * S::TILE);
+    unsigned char *sm_q = sm, *sm_k = sm + 2 * S::TILE, *sm_v = sm_k + KSLOTS * S::TILE;
+    Bars &fb = *reinterpret_cast<Bars *>(sm_v + VSLOTS * S::TILE);
     volatile int *abort = &fb.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -245,9 +246,13 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         tc::mbar_init(tc::smem_u32(&fb.q_full), 1);
         tc::mbar_init(tc::smem_u32(&fb.skew), 1);
         tc::mbar_init(tc::smem_u32(&fb.tail), 1);
-        for (int s = 0; s < SLOTS; ++s) {
-            tc::mbar_init(tc::smem_u32(&fb.full[s]), 1);
-            tc::mbar_init(tc::smem_u32(&fb.freed[s]), tiles);   // each tile's issuer
+        for (int s = 0; s < KSLOTS; ++s) {
+            tc::mbar_init(tc::smem_u32(&fb.k_full[s]), 1);
+            tc::mbar_init(tc::smem_u32(&fb.k_free[s]), tiles);   // each tile's score issuer
+        }
+        for (int s = 0; s < VSLOTS; ++s) {
+            tc::mbar_init(tc::smem_u32(&fb.v_full[s]), 1);
+            tc::mbar_init(tc::smem_u32(&fb.v_free[s]), tiles);   // each tile's value issuer
         }
         for (int i = 0; i < 2; ++i) {
             for (int b = 0; b < 2; ++b) {
@@ -256,6 +261,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 tc::mbar_init(tc::smem_u32(&fb.pv_done[i][b]), 1);
             }
             tc::mbar_init(tc::smem_u32(&fb.fin[i]), 1);
+            tc::mbar_init(tc::smem_u32(&fb.fin[2 + i]), 1);
         }
         fb.abort = 0;
         tc::fence_barrier_init();
@@ -263,7 +269,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         tc::prefetch_tmap(&kmap);
         tc::prefetch_tmap(&vmap);
     }
-    if (warp == 2 && nb) tc::tmem_alloc(tc::smem_u32(&fb.tmem), 512);
+    if (warp == 0 && nb) tc::tmem_alloc(tc::smem_u32(&fb.tmem), 512);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -293,13 +299,13 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         }
         int issued = 0;
         bool ok = true;
-        for (int f = 0; f < 2 * nb && ok; ++f) {
-            const int s = f % SLOTS, j = f >> 1;
-            if (f >= SLOTS) ok = tc::mbar_wait_abort(tc::smem_u32(&fb.freed[s]), ((f / SLOTS) - 1) & 1, abort, a.err, PK_FREE);
-            ok = __all_sync(0xffffffffu, ok);
+        for (int f = 0; f < 2 * nb && ok; ++f) {   // K_0, V_0, K_1, ...
+            const int j = f >> 1, v = f & 1, s = v ? j % VSLOTS : j % KSLOTS, turn = v ? j / VSLOTS : j / KSLOTS;
+            if (turn) ok = wait_all(v ? fb.v_free[s] : fb.k_free[s], turn - 1, abort, a.err, PK_FREE);
             if (!ok) break;
-            const CUtensorMap *map = (f & 1) ? &vmap : &kmap;
-            const uint32_t bar = tc::smem_u32(&fb.full[s]), dst = tc::smem_u32(sm_kv + s * S::TILE);
+            const CUtensorMap *map = v ? &vmap : &kmap;
+            const uint32_t bar = tc::smem_u32(v ? &fb.v_full[s] : &fb.k_full[s]);
+            const uint32_t dst = tc::smem_u32((v ? sm_v : sm_k) + s * S::TILE);
             const int key0 = kbeg + j * KB;
             const int boxes = a.prefix ? min(nbox, (kend - key0 + bt - 1) / bt) : 1;
             if (lane == 0) tc::mbar_arrive_expect_tx(bar, (uint32_t)(boxes * S::HALVES * bt * 128));
@@ -321,9 +327,9 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             issued = f + 1;
         }
         // the last block ends inside 16 keys: zero the rows of V behind its last key
-        const int nv = kend - kbeg - (nb - 1) * KB;
-        if (ok && (nv & 15) && wait_all(fb.full[(2 * nb - 1) % SLOTS], (2 * nb - 1) / SLOTS, abort, a.err, PK_KV)) {
-            unsigned char *v = sm_kv + ((2 * nb - 1) % SLOTS) * S::TILE + nv * 128;
+        const int nv = kend - kbeg - (nb - 1) * KB, sl = (nb - 1) % VSLOTS;
+        if (ok && (nv & 15) && wait_all(fb.v_full[sl], (nb - 1) / VSLOTS, abort, a.err, PK_KV)) {
+            unsigned char *v = sm_v + sl * S::TILE + nv * 128;
             const int words = (16 - (nv & 15)) * 8;
             for (int w = lane; w < words * S::HALVES; w += 32)
                 *reinterpret_cast<uint4 *>(v + (w / words) * BOX + (w % words) * 16) = make_uint4(0, 0, 0, 0);
@@ -334,53 +340,64 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         // copies in flight must land before the CTA's shared memory is released
         if (lane == 0) {
             tc::mbar_wait(tc::smem_u32(&fb.q_full), 0, nullptr, 0);
-            for (int f = issued > SLOTS ? issued - SLOTS : 0; f < issued; ++f)
-                tc::mbar_wait(tc::smem_u32(&fb.full[f % SLOTS]), (f / SLOTS) & 1, nullptr, 0);
+            for (int f = max(0, issued - 2 * VSLOTS); f < issued; ++f) {
+                const int j = f >> 1, v = f & 1;
+                if (!v && j + KSLOTS < (issued + 1) / 2) continue;   // filled again since
+                tc::mbar_wait(tc::smem_u32(v ? &fb.v_full[j % VSLOTS] : &fb.k_full[j % KSLOTS]), (v ? j / VSLOTS : j / KSLOTS) & 1, nullptr, 0);
+            }
         }
-    } else if ((warp == 1 || warp == 3) && nb && (warp >> 1) < tiles) {
-        // ---------------- MMA issuer of tile i (the whole warp waits, one lane issues) ----------------
-        // A warp for each tile: issuing and committing takes as long as the products,
-        // and one tile's waits must not hold up the other's products.
+    } else if ((warp == 3 || warp == 12) && nb && (warp == 3 || tiles == 2)) {
+        // ---------------- issuer of tile i's scores (the whole warp waits, one lane issues) ----------------
+        // Issuing, committing and waiting take as long as the products themselves: every
+        // chain of products has a warp of its own.
         constexpr uint32_t idesc_s = tc::idesc_f16_f32(TM, SB) | Pk<T>::fmt;
-        constexpr uint32_t idesc_pv = tc::idesc_f16_f32(TM, D) | (1u << 16) | Pk<T>::fmt;   // B (V) MN-major
-        const int i = warp >> 1;
+        const int i = warp == 3 ? 0 : 1;
         // descriptors differ only in their address field (16-byte units)
-        const uint64_t qd = tc::sdesc_k_sw128(tc::smem_u32(sm_q + i * S::TILE)), kd0 = tc::sdesc_k_sw128(tc::smem_u32(sm_kv));
-        const uint64_t vd0 = tc::sdesc_mn_sw128(tc::smem_u32(sm_kv), BOX);
-        const uint32_t tS = tmem + COL_S + i * 128, tO = tmem + COL_O + i * 128;
-        auto slot_wait = [&](int f) { return wait_all(fb.full[f % SLOTS], f / SLOTS, abort, a.err, PK_KV); };
-        // scores of keys 64 n .. 64 n + 63 into buffer n & 1
-        auto issue_s = [&](int n) {
+        const uint64_t qd = tc::sdesc_k_sw128(tc::smem_u32(sm_q + i * S::TILE)), kd0 = tc::sdesc_k_sw128(tc::smem_u32(sm_k));
+        const uint32_t tS = tmem + COL_S + i * 128;
+        bool ok = wait_all(fb.q_full, 0, abort, a.err, PK_Q);
+        // tile 1 starts when tile 0 is through its first scores, so that the one's
+        // softmax meets the other's products from then on
+        if (i) ok = ok && wait_all(fb.skew, 0, abort, a.err, PK_P);
+        // keys 64 n .. 64 n + 63 into buffer n & 1
+        for (int n = 0; n < ns && ok; ++n) {
+            const int b = n & 1, j = n >> 1, sl = j % KSLOTS;
+            if (!b) ok = wait_all(fb.k_full[sl], j / KSLOTS, abort, a.err, PK_KV);
+            // the scores lie over P of block n - 2: the product that reads it comes first
+            if (n >= 2) ok = ok && wait_all(fb.pv_done[i][b], j - 1, abort, a.err, PK_PV);
+            if (!ok) break;
             tc::fence_after_sync();
-            const uint64_t kd = kd0 + (uint32_t)(((n & ~1) % SLOTS) * (S::TILE >> 4) + (n & 1) * (SB * 128 >> 4));
-            const uint32_t d = tS + (n & 1) * SB;
+            const uint64_t kd = kd0 + (uint32_t)(sl * (S::TILE >> 4) + b * (SB * 128 >> 4));
+            const uint32_t d = tS + b * SB;
             if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t off = (uint32_t)(((kk >> 2) * BOX + (kk & 3) * 32) >> 4);
                     tc::mma_ss_f16(d, qd + off, kd + off, idesc_s, kk ? 1u : 0u);
                 }
-                tc::mma_commit(tc::smem_u32(&fb.s_full[i][n & 1]));
+                tc::mma_commit(tc::smem_u32(&fb.s_full[i][b]));
+                if (b) tc::mma_commit(tc::smem_u32(&fb.k_free[sl]));
             }
             __syncwarp();
-        };
-        bool ok = wait_all(fb.q_full, 0, abort, a.err, PK_Q) && slot_wait(0);
-        // tile 1 starts when tile 0 is through its first scores, so that the one's
-        // softmax meets the other's products from the start
-        if (i) ok = ok && wait_all(fb.skew, 0, abort, a.err, PK_P);
-        if (ok) {
-            issue_s(0);
-            if (ns > 1) issue_s(1);
-            if (elect_one()) tc::mma_commit(tc::smem_u32(&fb.freed[0]));
-            __syncwarp();
         }
+        // everything issued must finish before TMEM is freed
+        if (elect_one()) tc::mma_commit(tc::smem_u32(&fb.fin[2 + i]));
+        __syncwarp();
+        tc::mbar_wait(tc::smem_u32(&fb.fin[2 + i]), 0, nullptr, 0);
+    } else if ((warp == 1 || warp == 2) && nb && warp <= tiles) {
+        // ---------------- issuer of tile i's O += P V ----------------
+        constexpr uint32_t idesc_pv = tc::idesc_f16_f32(TM, D) | (1u << 16) | Pk<T>::fmt;   // B (V) MN-major
+        const int i = warp - 1;
+        const uint64_t vd0 = tc::sdesc_mn_sw128(tc::smem_u32(sm_v), BOX);
+        const uint32_t tS = tmem + COL_S + i * 128, tO = tmem + COL_O + i * 128;
+        bool ok = true;
         for (int n = 0; n < ns && ok; ++n) {
-            const int b = n & 1, fk = n & ~1, fv = fk + 1;   // ring fills of the block's K and V
-            const uint64_t vd = vd0 + (uint32_t)((fv % SLOTS) * (S::TILE >> 4) + b * (SB * 128 >> 4));
-            const int nv = min(SB, kend - kbeg - n * SB), ks = (nv + 15) / 16;   // 16-key steps that hold keys
-            ok = slot_wait(fv);
+            const int b = n & 1, j = n >> 1, sl = j % VSLOTS;
+            const uint64_t vd = vd0 + (uint32_t)(sl * (S::TILE >> 4) + b * (SB * 128 >> 4));
+            const int nv = n + 1 < ns ? SB : kend - kbeg - n * SB, ks = (nv + 15) / 16;   // 16-key steps that hold keys
+            if (!b) ok = wait_all(fb.v_full[sl], j / VSLOTS, abort, a.err, PK_KV);
             if (nv & 15) ok = ok && wait_all(fb.tail, 0, abort, a.err, PK_KV);   // the rows behind the last key are zeroed
-            ok = ok && wait_all(fb.p_full[i][b], n >> 1, abort, a.err, PK_P);
+            ok = ok && wait_all(fb.p_full[i][b], j, abort, a.err, PK_P);
             if (!ok) break;
             tc::fence_after_sync();
             if (elect_one()) {
@@ -393,24 +410,14 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                         tc::mma_ts_f16(tO, tS + b * SB + kk * 8, vd + kk * 128, idesc_pv, (n | kk) ? 1u : 0u);
                 }
                 tc::mma_commit(tc::smem_u32(&fb.pv_done[i][b]));
-            }
-            __syncwarp();
-            if (n + 2 < ns) {
-                // the next scores of this buffer lie over P: the product that reads P comes first
-                ok = slot_wait(fk + 2) && wait_all(fb.pv_done[i][b], n >> 1, abort, a.err, PK_PV);
-                if (ok) issue_s(n + 2);
-            }
-            if (ok && b && elect_one()) {   // the block's V, and the next block's K, are no longer needed here
-                tc::mma_commit(tc::smem_u32(&fb.freed[fv % SLOTS]));
-                if (n + 2 < ns) tc::mma_commit(tc::smem_u32(&fb.freed[(fk + 2) % SLOTS]));
+                if (b) tc::mma_commit(tc::smem_u32(&fb.v_free[sl]));   // the block's V is no longer needed here
             }
             __syncwarp();
         }
-        // everything issued must finish before TMEM is freed
         if (elect_one()) tc::mma_commit(tc::smem_u32(&fb.fin[i]));
         __syncwarp();
         tc::mbar_wait(tc::smem_u32(&fb.fin[i]), 0, nullptr, 0);
-    } else if (warp >= 4 && any) {
+    } else if (warp >= 4 && warp < 12 && any) {
         // ---------------- softmax and epilogue: thread = query row ----------------
         const int i = (warp - 4) >> 2, quarter = warp & 3;
         if (i < tiles) {
@@ -539,7 +546,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == 2 && nb) {
+    if (warp == 0 && nb) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, 512);
     }
