@@ -2,7 +2,10 @@
 // rows: causal attention of packed prompts, and the pass of a whole batch over
 // the keys of a shared prefix.
 //
-// CTA = up to two tiles of 128 query rows of one KV head.  A row is a (token,
+// Item of work = up to two tiles of 128 query rows of one KV head; a CTA takes one
+// after the other (the next one's number comes from cluster launch control: a CTA
+// that would have started later is cancelled and its item done here), so that the
+// start of an item overlaps the end of the one before.  A row is a (token,
 // query head of the group) pair, token-major, so all G heads that share a KV
 // head read its tiles once and a short sequence still fills rows.  Keys stream
 // in blocks of 128 through a ring of shared-memory slots (K_0, V_0, K_1, ...).
@@ -52,11 +55,22 @@ constexpr int THREADS = 416;
 constexpr int SB = 64;                  // keys of a score buffer: two per tile
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
-enum PkErr { PK_Q = 61, PK_KV, PK_FREE, PK_S, PK_P, PK_PV, PK_ALIGN };
+enum PkErr { PK_Q = 61, PK_KV, PK_FREE, PK_S, PK_P, PK_PV, PK_ALIGN, PK_WORK };
+
+// One item of work: up to two tiles of query tokens [tok0, tok0 + ntok) of KV head
+// h against keys [kbeg, kend) of a sequence (counted from its start).
+struct Work {
+    int end;                    // no more items
+    int tok0, ntok, kbeg, kend, krow0, first_lim, split, h;
+    int nb, ns, tiles;          // key blocks, score blocks, tiles
+};
 
 struct Bars {
-    unsigned long long q_full, k_full[KSLOTS], k_free[KSLOTS], v_full[VSLOTS], v_free[VSLOTS], skew, tail, fin[4];
+    unsigned long long q_full[2], q_free[2], k_full[KSLOTS], k_free[KSLOTS], v_full[VSLOTS], v_free[VSLOTS];
     unsigned long long s_full[2][2], p_full[2][2], pv_done[2][2];   // [tile][score buffer]
+    unsigned long long o_free[2], work_full[2], work_free[2], next, v_part, skew, fin[4];
+    __align__(16) uint32_t response[4];   // of the request for the next item
+    Work work[2];
     uint32_t tmem;
     int abort;
 };
@@ -172,6 +186,75 @@ struct Pk<__nv_bfloat16> {
     }
 };
 
+// Ask the launch for a CTA that has not started (cluster launch control): it will
+// not start, and its number arrives in 16 bytes of shared memory.
+__device__ __forceinline__ void request_next(uint32_t response, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(response), "r"(bar)
+                 : "memory");
+}
+// false: every CTA has started
+__device__ __forceinline__ bool next_item(uint32_t response, int *id) {
+    uint32_t got, x;
+    asm volatile(
+        "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}\n"
+        : "=r"(got), "=r"(x)
+        : "r"(response)
+        : "memory");
+    if (got) *id = (int)x;
+    // the response is written again by the async proxy
+    tc::fence_proxy_async_smem();
+    return got != 0;
+}
+
+// Item `id` of the grid; ntok <= 0: none there.
+__device__ __forceinline__ Work work_of(const Args &a, int id) {
+    Work w = {};
+    w.h = id % a.Hkv;
+    const int x = id / a.Hkv;
+    if (!a.prefix) {
+        // sequence s owns tile numbers from cu_q[s] / (2 TQ) + s on: one more than
+        // its tokens need at most, so the map needs no prefix sum
+        const int tile = gridDim.x / a.Hkv - 1 - x;   // the last tiles see most keys: first
+        int lo = 0, hi = a.n_seq - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (__ldg(a.cu_q + mid) / (2 * a.TQ) + mid <= tile) lo = mid;
+            else hi = mid - 1;
+        }
+        // offsets outside the buffers are cut to them
+        const int q0 = min(max(__ldg(a.cu_q + lo), 0), a.Tq), q1 = min(max(__ldg(a.cu_q + lo + 1), q0), a.Tq);
+        const int k0 = min(max(__ldg(a.cu_k + lo), 0), a.Tk), k1 = min(max(__ldg(a.cu_k + lo + 1), k0), a.Tk);
+        const int at = (tile - (__ldg(a.cu_q + lo) / (2 * a.TQ) + lo)) * 2 * a.TQ;   // token of the sequence
+        if (at >= 0 && at < q1 - q0) {
+            w.tok0 = q0 + at;
+            w.ntok = min(2 * a.TQ, q1 - w.tok0);
+        }
+        w.krow0 = k0;
+        const int nk = k1 - k0, nq = q1 - q0;
+        w.first_lim = a.causal ? nk - nq + at : nk - 1;
+        w.kend = a.causal ? min(nk, w.first_lim + w.ntok) : nk;   // one past the last key any row sees
+    } else {
+        const int pairs = (a.M + 2 * a.TQ - 1) / (2 * a.TQ);
+        w.split = x / pairs;
+        w.tok0 = (x % pairs) * 2 * a.TQ;
+        w.ntok = min(2 * a.TQ, a.M - w.tok0);
+        const int blocks = (a.prefix_len + KB - 1) / KB;
+        w.kbeg = (int)((int64_t)blocks * w.split / a.splits) * KB;
+        w.kend = min(a.prefix_len, (int)((int64_t)blocks * (w.split + 1) / a.splits) * KB);
+    }
+    if (w.ntok > 0 && w.kend > w.kbeg) {
+        w.nb = (w.kend - w.kbeg + KB - 1) / KB;
+        w.ns = (w.kend - w.kbeg + SB - 1) / SB;
+    }
+    w.tiles = w.ntok > a.TQ ? 2 : 1;
+    return w;
+}
+
 // The whole warp waits for phase `n` of a barrier: false when it ran out of time
 // or the CTA has been given up.
 __device__ __forceinline__ bool wait_all(unsigned long long &bar, int n, volatile int *abort, int32_t *err, int code) {
@@ -202,57 +285,14 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     griddep_wait();
     griddep_launch_dependents();
 
-    // ---- which tokens and keys: tokens [tok0, tok0 + ntok) of the packed
-    // queries, keys [kbeg, kend) counted from the sequence's start
-    const int h = blockIdx.x % a.Hkv;
-    int tok0 = 0, ntok = 0, kbeg = 0, kend = 0, krow0 = 0, first_lim = 0, split = 0;
-    if (!a.prefix) {
-        // sequence s owns tile numbers from cu_q[s] / (2 TQ) + s on: one more than
-        // its tokens need at most, so the map needs no prefix sum
-        const int tile = gridDim.x / a.Hkv - 1 - blockIdx.x / a.Hkv;   // the last tiles see most keys: first
-        int lo = 0, hi = a.n_seq - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (__ldg(a.cu_q + mid) / (2 * a.TQ) + mid <= tile) lo = mid;
-            else hi = mid - 1;
-        }
-        // offsets outside the buffers are cut to them
-        const int q0 = min(max(__ldg(a.cu_q + lo), 0), a.Tq), q1 = min(max(__ldg(a.cu_q + lo + 1), q0), a.Tq);
-        const int k0 = min(max(__ldg(a.cu_k + lo), 0), a.Tk), k1 = min(max(__ldg(a.cu_k + lo + 1), k0), a.Tk);
-        const int at = (tile - (__ldg(a.cu_q + lo) / (2 * a.TQ) + lo)) * 2 * a.TQ;   // token of the sequence
-        if (at >= 0 && at < q1 - q0) {
-            tok0 = q0 + at;
-            ntok = min(2 * a.TQ, q1 - tok0);
-        }
-        krow0 = k0;
-        const int nk = k1 - k0, nq = q1 - q0;
-        first_lim = a.causal ? nk - nq + at : nk - 1;
-        kend = a.causal ? min(nk, first_lim + ntok) : nk;   // one past the last key any row sees
-    } else {
-        const int pairs = (a.M + 2 * a.TQ - 1) / (2 * a.TQ), x = blockIdx.x / a.Hkv;
-        split = x / pairs;
-        tok0 = (x % pairs) * 2 * a.TQ;
-        ntok = min(2 * a.TQ, a.M - tok0);
-        const int blocks = (a.prefix_len + KB - 1) / KB;
-        kbeg = (int)((int64_t)blocks * split / a.splits) * KB;
-        kend = min(a.prefix_len, (int)((int64_t)blocks * (split + 1) / a.splits) * KB);
-    }
-    const bool any = ntok > 0;
-    const int nb = any && kend > kbeg ? (kend - kbeg + KB - 1) / KB : 0;
-    const int ns = nb ? (kend - kbeg + SB - 1) / SB : 0;   // score blocks
-    const int tiles = ntok > a.TQ ? 2 : 1;
-
     if (threadIdx.x == 0) {
-        tc::mbar_init(tc::smem_u32(&fb.q_full), 1);
-        tc::mbar_init(tc::smem_u32(&fb.skew), 1);
-        tc::mbar_init(tc::smem_u32(&fb.tail), 1);
         for (int s = 0; s < KSLOTS; ++s) {
             tc::mbar_init(tc::smem_u32(&fb.k_full[s]), 1);
-            tc::mbar_init(tc::smem_u32(&fb.k_free[s]), tiles);   // each tile's score issuer
+            tc::mbar_init(tc::smem_u32(&fb.k_free[s]), 2);   // each tile's score issuer
         }
         for (int s = 0; s < VSLOTS; ++s) {
             tc::mbar_init(tc::smem_u32(&fb.v_full[s]), 1);
-            tc::mbar_init(tc::smem_u32(&fb.v_free[s]), tiles);   // each tile's value issuer
+            tc::mbar_init(tc::smem_u32(&fb.v_free[s]), 2);   // each tile's value issuer
         }
         for (int i = 0; i < 2; ++i) {
             for (int b = 0; b < 2; ++b) {
@@ -260,30 +300,41 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 tc::mbar_init(tc::smem_u32(&fb.p_full[i][b]), 4);   // the tile's softmax warps
                 tc::mbar_init(tc::smem_u32(&fb.pv_done[i][b]), 1);
             }
+            tc::mbar_init(tc::smem_u32(&fb.q_full[i]), 1);
+            tc::mbar_init(tc::smem_u32(&fb.q_free[i]), 1);
+            tc::mbar_init(tc::smem_u32(&fb.o_free[i]), 4);
+            tc::mbar_init(tc::smem_u32(&fb.work_full[i]), 1);
+            tc::mbar_init(tc::smem_u32(&fb.work_free[i]), 12);      // every warp but the producer
             tc::mbar_init(tc::smem_u32(&fb.fin[i]), 1);
             tc::mbar_init(tc::smem_u32(&fb.fin[2 + i]), 1);
         }
+        tc::mbar_init(tc::smem_u32(&fb.next), 1);
+        tc::mbar_init(tc::smem_u32(&fb.v_part), 1);
+        tc::mbar_init(tc::smem_u32(&fb.skew), 1);
         fb.abort = 0;
         tc::fence_barrier_init();
         tc::prefetch_tmap(&qmap);
         tc::prefetch_tmap(&kmap);
         tc::prefetch_tmap(&vmap);
     }
-    if (warp == 0 && nb) tc::tmem_alloc(tc::smem_u32(&fb.tmem), 512);
+    if (warp == 0) tc::tmem_alloc(tc::smem_u32(&fb.tmem), 512);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = fb.tmem;
 
-    if (warp == 0 && nb) {
-        // ---------------- TMA producer ----------------
-        if (lane == 0) {
-            const uint32_t qb = tc::smem_u32(&fb.q_full);
-            tc::mbar_arrive_expect_tx(qb, (uint32_t)(tiles * S::HALVES * a.G * a.TQ * 128));
-            for (int i = 0; i < tiles; ++i)
-                for (int x = 0; x < S::HALVES; ++x)
-                    tc::tma_load_3d(tc::smem_u32(sm_q + i * S::TILE + x * BOX), &qmap, x * 64, h * a.G, tok0 + i * a.TQ, qb);
-        }
+    // The next item of a reading warp (all but the producer): its number, then what
+    // it is.  False at the end, or when the CTA has been given up.
+    auto next_work = [&](int it, Work &w) -> bool {
+        if (!wait_all(fb.work_full[it & 1], it >> 1, abort, a.err, PK_WORK)) return false;
+        w = fb.work[it & 1];
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.work_free[it & 1]));
+        return !w.end;
+    };
+
+    if (warp == 0) {
+        // ---------------- items and TMA producer ----------------
         // boxes of a block: `bt` tokens each (a page, or all 128 keys)
         const int bt = a.prefix ? min(KB, 1 << a.kv.page_shift) : KB, nbox = KB / bt;
         const int32_t *table = nullptr;
@@ -297,56 +348,102 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             }
             table = row < 0 ? nullptr : a.kv.table + (size_t)row * a.kv.max_pages;
         }
-        int issued = 0;
-        bool ok = true;
-        for (int f = 0; f < 2 * nb && ok; ++f) {   // K_0, V_0, K_1, ...
-            const int j = f >> 1, v = f & 1, s = v ? j % VSLOTS : j % KSLOTS, turn = v ? j / VSLOTS : j / KSLOTS;
-            if (turn) ok = wait_all(v ? fb.v_free[s] : fb.k_free[s], turn - 1, abort, a.err, PK_FREE);
-            if (!ok) break;
-            const CUtensorMap *map = v ? &vmap : &kmap;
-            const uint32_t bar = tc::smem_u32(v ? &fb.v_full[s] : &fb.k_full[s]);
-            const uint32_t dst = tc::smem_u32((v ? sm_v : sm_k) + s * S::TILE);
-            const int key0 = kbeg + j * KB;
-            const int boxes = a.prefix ? min(nbox, (kend - key0 + bt - 1) / bt) : 1;
-            if (lane == 0) tc::mbar_arrive_expect_tx(bar, (uint32_t)(boxes * S::HALVES * bt * 128));
+        bool ok = true, more = true;
+        int it = 0, asked = 0, kc = 0, vc = 0, vp = 0, qc0 = 0, qc1 = 0;   // items shown, requests, fills so far
+        for (int id = blockIdx.x; ok; ++asked) {
+            // ask for the CTA that would start next (its item becomes this CTA's); the
+            // answer is read when this item's copies have been issued
+            if (lane == 0) {
+                tc::mbar_arrive_expect_tx(tc::smem_u32(&fb.next), 16);
+                request_next(tc::smem_u32(fb.response), tc::smem_u32(&fb.next));
+            }
             __syncwarp();
-            if (lane < boxes * S::HALVES) {
-                const int b = lane / S::HALVES, x = lane % S::HALVES;
-                if (a.prefix) {
-                    const int key = key0 + b * bt;
-                    int page = table ? __ldg(table + (key >> a.kv.page_shift)) : -1;
-                    if (page < 0 || page >= a.kv.n_pages) {   // reads as zeros (a box outside the tensor)
-                        if (table && a.err) atomicExch(a.err, PE_PAGE);
-                        page = a.kv.n_pages;
+            const Work w = work_of(a, id);
+            if (w.ntok > 0) {
+                if (it >= 2) ok = wait_all(fb.work_free[it & 1], (it >> 1) - 1, abort, a.err, PK_WORK);
+                if (ok && lane == 0) {
+                    fb.work[it & 1] = w;
+                    tc::mbar_arrive(tc::smem_u32(&fb.work_full[it & 1]));
+                }
+                ++it;
+            }
+            if (w.ntok > 0 && w.nb) {
+                for (int i = 0; i < w.tiles && ok; ++i) {
+                    int &qc = i ? qc1 : qc0;
+                    if (qc) ok = wait_all(fb.q_free[i], qc - 1, abort, a.err, PK_FREE);
+                    if (ok && lane == 0) {
+                        const uint32_t qb = tc::smem_u32(&fb.q_full[i]);
+                        tc::mbar_arrive_expect_tx(qb, (uint32_t)(S::HALVES * a.G * a.TQ * 128));
+                        for (int x = 0; x < S::HALVES; ++x)
+                            tc::tma_load_3d(tc::smem_u32(sm_q + i * S::TILE + x * BOX), &qmap, x * 64, w.h * a.G, w.tok0 + i * a.TQ, qb);
                     }
-                    tma_load_4d(dst + x * BOX + b * bt * 128, map, x * 64, key & ((1 << a.kv.page_shift) - 1), h, page, bar);
-                } else {
-                    tma_load_4d(dst + x * BOX, map, x * 64, krow0 + key0, h, 0, bar);
+                    if (ok) ++qc;
+                }
+                for (int f = 0; f < 2 * w.nb && ok; ++f) {   // K_0, V_0, K_1, ...
+                    const int j = f >> 1, v = f & 1, fill = v ? vc : kc, s = v ? fill % VSLOTS : fill % KSLOTS, turn = v ? fill / VSLOTS : fill / KSLOTS;
+                    if (turn) ok = wait_all(v ? fb.v_free[s] : fb.k_free[s], turn - 1, abort, a.err, PK_FREE);
+                    if (!ok) break;
+                    const int key0 = w.kbeg + j * KB, nv = w.kend - key0;
+                    // V of a block that ends inside 16 keys is shown only when the rows behind
+                    // its last key are zeroed
+                    const bool part = v && j + 1 == w.nb && (nv & 15);
+                    const CUtensorMap *map = v ? &vmap : &kmap;
+                    const uint32_t bar = tc::smem_u32(part ? &fb.v_part : v ? &fb.v_full[s] : &fb.k_full[s]);
+                    unsigned char *tile = (v ? sm_v : sm_k) + s * S::TILE;
+                    const uint32_t dst = tc::smem_u32(tile);
+                    const int boxes = a.prefix ? min(nbox, (nv + bt - 1) / bt) : 1;
+                    if (lane == 0) tc::mbar_arrive_expect_tx(bar, (uint32_t)(boxes * S::HALVES * bt * 128));
+                    __syncwarp();
+                    if (lane < boxes * S::HALVES) {
+                        const int b = lane / S::HALVES, x = lane % S::HALVES;
+                        if (a.prefix) {
+                            const int key = key0 + b * bt;
+                            int page = table ? __ldg(table + (key >> a.kv.page_shift)) : -1;
+                            if (page < 0 || page >= a.kv.n_pages) {   // reads as zeros (a box outside the tensor)
+                                if (table && a.err) atomicExch(a.err, PE_PAGE);
+                                page = a.kv.n_pages;
+                            }
+                            tma_load_4d(dst + x * BOX + b * bt * 128, map, x * 64, key & ((1 << a.kv.page_shift) - 1), w.h, page, bar);
+                        } else {
+                            tma_load_4d(dst + x * BOX, map, x * 64, w.krow0 + key0, w.h, 0, bar);
+                        }
+                    }
+                    if (v) ++vc;
+                    else ++kc;
+                    if (part) {
+                        ok = wait_all(fb.v_part, vp++, abort, a.err, PK_KV);
+                        if (!ok) break;
+                        const int words = (16 - (nv & 15)) * 8;
+                        for (int y = lane; y < words * S::HALVES; y += 32)
+                            *reinterpret_cast<uint4 *>(tile + (y / words) * BOX + nv * 128 + (y % words) * 16) = make_uint4(0, 0, 0, 0);
+                        tc::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.v_full[s]));
+                    }
                 }
             }
-            issued = f + 1;
-        }
-        // the last block ends inside 16 keys: zero the rows of V behind its last key
-        const int nv = kend - kbeg - (nb - 1) * KB, sl = (nb - 1) % VSLOTS;
-        if (ok && (nv & 15) && wait_all(fb.v_full[sl], (nb - 1) / VSLOTS, abort, a.err, PK_KV)) {
-            unsigned char *v = sm_v + sl * S::TILE + nv * 128;
-            const int words = (16 - (nv & 15)) * 8;
-            for (int w = lane; w < words * S::HALVES; w += 32)
-                *reinterpret_cast<uint4 *>(v + (w / words) * BOX + (w % words) * 16) = make_uint4(0, 0, 0, 0);
-            tc::fence_proxy_async_smem();
+            // the answer; it must be in before the CTA ends, whatever else happened
+            const bool in = tc::mbar_wait(tc::smem_u32(&fb.next), asked & 1, a.err, PK_WORK);
+            more = __all_sync(0xffffffffu, in) && next_item(tc::smem_u32(fb.response), &id);
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.tail));
+            if (!more) break;
         }
-        // copies in flight must land before the CTA's shared memory is released
-        if (lane == 0) {
-            tc::mbar_wait(tc::smem_u32(&fb.q_full), 0, nullptr, 0);
-            for (int f = max(0, issued - 2 * VSLOTS); f < issued; ++f) {
-                const int j = f >> 1, v = f & 1;
-                if (!v && j + KSLOTS < (issued + 1) / 2) continue;   // filled again since
-                tc::mbar_wait(tc::smem_u32(v ? &fb.v_full[j % VSLOTS] : &fb.k_full[j % KSLOTS]), (v ? j / VSLOTS : j / KSLOTS) & 1, nullptr, 0);
+        if (ok) {   // show the end
+            if (it >= 2) ok = wait_all(fb.work_free[it & 1], (it >> 1) - 1, abort, a.err, PK_WORK);
+            if (ok && lane == 0) {
+                fb.work[it & 1].end = 1;
+                tc::mbar_arrive(tc::smem_u32(&fb.work_full[it & 1]));
             }
         }
-    } else if ((warp == 3 || warp == 12) && nb && (warp == 3 || tiles == 2)) {
+        // copies in flight must land before the CTA's shared memory is released
+        if (*abort) {
+            if (qc0) tc::mbar_wait(tc::smem_u32(&fb.q_full[0]), (qc0 - 1) & 1, nullptr, 0);
+            if (qc1) tc::mbar_wait(tc::smem_u32(&fb.q_full[1]), (qc1 - 1) & 1, nullptr, 0);
+            for (int f = max(0, kc - KSLOTS); f < kc; ++f) tc::mbar_wait(tc::smem_u32(&fb.k_full[f % KSLOTS]), (f / KSLOTS) & 1, nullptr, 0);
+            for (int f = max(0, vc - VSLOTS); f < vc; ++f) tc::mbar_wait(tc::smem_u32(&fb.v_full[f % VSLOTS]), (f / VSLOTS) & 1, nullptr, 0);
+            if (vp) tc::mbar_wait(tc::smem_u32(&fb.v_part), (vp - 1) & 1, nullptr, 0);
+        }
+    } else if (warp == 3 || warp == 12) {
         // ---------------- issuer of tile i's scores (the whole warp waits, one lane issues) ----------------
         // Issuing, committing and waiting take as long as the products themselves: every
         // chain of products has a warp of its own.
@@ -355,91 +452,128 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         // descriptors differ only in their address field (16-byte units)
         const uint64_t qd = tc::sdesc_k_sw128(tc::smem_u32(sm_q + i * S::TILE)), kd0 = tc::sdesc_k_sw128(tc::smem_u32(sm_k));
         const uint32_t tS = tmem + COL_S + i * 128;
-        bool ok = wait_all(fb.q_full, 0, abort, a.err, PK_Q);
-        // tile 1 starts when tile 0 is through its first scores, so that the one's
-        // softmax meets the other's products from then on
-        if (i) ok = ok && wait_all(fb.skew, 0, abort, a.err, PK_P);
-        // keys 64 n .. 64 n + 63 into buffer n & 1
-        for (int n = 0; n < ns && ok; ++n) {
-            const int b = n & 1, j = n >> 1, sl = j % KSLOTS;
-            if (!b) ok = wait_all(fb.k_full[sl], j / KSLOTS, abort, a.err, PK_KV);
-            // the scores lie over P of block n - 2: the product that reads it comes first
-            if (n >= 2) ok = ok && wait_all(fb.pv_done[i][b], j - 1, abort, a.err, PK_PV);
-            if (!ok) break;
-            tc::fence_after_sync();
-            const uint64_t kd = kd0 + (uint32_t)(sl * (S::TILE >> 4) + b * (SB * 128 >> 4));
-            const uint32_t d = tS + b * SB;
-            if (elect_one()) {
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (uint32_t)(((kk >> 2) * BOX + (kk & 3) * 32) >> 4);
-                    tc::mma_ss_f16(d, qd + off, kd + off, idesc_s, kk ? 1u : 0u);
-                }
-                tc::mma_commit(tc::smem_u32(&fb.s_full[i][b]));
-                if (b) tc::mma_commit(tc::smem_u32(&fb.k_free[sl]));
+        bool ok = true;
+        Work w;
+        // blocks of K and scores of this tile so far, items with scores
+        for (int it = 0, kc = 0, sc = 0, qc = 0; ok && next_work(it, w); ++it) {
+            if (i >= w.tiles || !w.nb) {
+                kc += w.nb;
+                continue;
             }
-            __syncwarp();
+            ok = wait_all(fb.q_full[i], qc++, abort, a.err, PK_Q);
+            // tile 1 starts when tile 0 is through its first scores, so that the one's
+            // softmax meets the other's products from then on
+            if (i && !it) ok = ok && wait_all(fb.skew, 0, abort, a.err, PK_P);
+            for (int n = 0; n < w.ns && ok; ++n, ++sc) {   // keys 64 n .. 64 n + 63 into buffer sc & 1
+                const int half = n & 1, b = sc & 1, kb = kc + (n >> 1), sl = kb % KSLOTS;
+                if (!half) ok = wait_all(fb.k_full[sl], kb / KSLOTS, abort, a.err, PK_KV);
+                // the scores lie over P of two blocks ago: the product that reads it comes first
+                if (sc >= 2) ok = ok && wait_all(fb.pv_done[i][b], (sc >> 1) - 1, abort, a.err, PK_PV);
+                if (!ok) break;
+                tc::fence_after_sync();
+                const uint64_t kd = kd0 + (uint32_t)(sl * (S::TILE >> 4) + half * (SB * 128 >> 4));
+                const uint32_t d = tS + b * SB;
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (uint32_t)(((kk >> 2) * BOX + (kk & 3) * 32) >> 4);
+                        tc::mma_ss_f16(d, qd + off, kd + off, idesc_s, kk ? 1u : 0u);
+                    }
+                    tc::mma_commit(tc::smem_u32(&fb.s_full[i][b]));
+                    if (half || n + 1 == w.ns) {
+                        tc::mma_commit(tc::smem_u32(&fb.k_free[sl]));
+                        if (w.tiles == 1) tc::mma_commit(tc::smem_u32(&fb.k_free[sl]));   // for the tile that is not there
+                    }
+                    if (n + 1 == w.ns) tc::mma_commit(tc::smem_u32(&fb.q_free[i]));
+                }
+                __syncwarp();
+            }
+            kc += w.nb;
         }
         // everything issued must finish before TMEM is freed
         if (elect_one()) tc::mma_commit(tc::smem_u32(&fb.fin[2 + i]));
         __syncwarp();
         tc::mbar_wait(tc::smem_u32(&fb.fin[2 + i]), 0, nullptr, 0);
-    } else if ((warp == 1 || warp == 2) && nb && warp <= tiles) {
+    } else if (warp == 1 || warp == 2) {
         // ---------------- issuer of tile i's O += P V ----------------
         constexpr uint32_t idesc_pv = tc::idesc_f16_f32(TM, D) | (1u << 16) | Pk<T>::fmt;   // B (V) MN-major
         const int i = warp - 1;
         const uint64_t vd0 = tc::sdesc_mn_sw128(tc::smem_u32(sm_v), BOX);
         const uint32_t tS = tmem + COL_S + i * 128, tO = tmem + COL_O + i * 128;
         bool ok = true;
-        for (int n = 0; n < ns && ok; ++n) {
-            const int b = n & 1, j = n >> 1, sl = j % VSLOTS;
-            const uint64_t vd = vd0 + (uint32_t)(sl * (S::TILE >> 4) + b * (SB * 128 >> 4));
-            const int nv = n + 1 < ns ? SB : kend - kbeg - n * SB, ks = (nv + 15) / 16;   // 16-key steps that hold keys
-            if (!b) ok = wait_all(fb.v_full[sl], j / VSLOTS, abort, a.err, PK_KV);
-            if (nv & 15) ok = ok && wait_all(fb.tail, 0, abort, a.err, PK_KV);   // the rows behind the last key are zeroed
-            ok = ok && wait_all(fb.p_full[i][b], j, abort, a.err, PK_P);
-            if (!ok) break;
-            tc::fence_after_sync();
-            if (elect_one()) {
-                if (ks == SB / 16) {
-#pragma unroll
-                    for (int kk = 0; kk < SB / 16; ++kk)
-                        tc::mma_ts_f16(tO, tS + b * SB + kk * 8, vd + kk * 128, idesc_pv, (n | kk) ? 1u : 0u);
-                } else {
-                    for (int kk = 0; kk < ks; ++kk)
-                        tc::mma_ts_f16(tO, tS + b * SB + kk * 8, vd + kk * 128, idesc_pv, (n | kk) ? 1u : 0u);
-                }
-                tc::mma_commit(tc::smem_u32(&fb.pv_done[i][b]));
-                if (b) tc::mma_commit(tc::smem_u32(&fb.v_free[sl]));   // the block's V is no longer needed here
+        Work w;
+        for (int it = 0, vc = 0, sc = 0, oc = 0; ok && next_work(it, w); ++it) {
+            if (i >= w.tiles || !w.nb) {
+                vc += w.nb;
+                continue;
             }
-            __syncwarp();
+            if (oc) ok = wait_all(fb.o_free[i], oc - 1, abort, a.err, PK_PV);   // the last item's O has been read
+            ++oc;
+            for (int n = 0; n < w.ns && ok; ++n, ++sc) {
+                const int half = n & 1, b = sc & 1, vb = vc + (n >> 1), sl = vb % VSLOTS;
+                const uint64_t vd = vd0 + (uint32_t)(sl * (S::TILE >> 4) + half * (SB * 128 >> 4));
+                const int nv = n + 1 < w.ns ? SB : w.kend - w.kbeg - n * SB, ks = (nv + 15) / 16;   // 16-key steps that hold keys
+                if (!half) ok = wait_all(fb.v_full[sl], vb / VSLOTS, abort, a.err, PK_KV);
+                ok = ok && wait_all(fb.p_full[i][b], sc >> 1, abort, a.err, PK_P);
+                if (!ok) break;
+                tc::fence_after_sync();
+                if (elect_one()) {
+                    if (ks == SB / 16) {
+#pragma unroll
+                        for (int kk = 0; kk < SB / 16; ++kk)
+                            tc::mma_ts_f16(tO, tS + b * SB + kk * 8, vd + kk * 128, idesc_pv, (n | kk) ? 1u : 0u);
+                    } else {
+                        for (int kk = 0; kk < ks; ++kk)
+                            tc::mma_ts_f16(tO, tS + b * SB + kk * 8, vd + kk * 128, idesc_pv, (n | kk) ? 1u : 0u);
+                    }
+                    tc::mma_commit(tc::smem_u32(&fb.pv_done[i][b]));
+                    if (half || n + 1 == w.ns) {
+                        tc::mma_commit(tc::smem_u32(&fb.v_free[sl]));
+                        if (w.tiles == 1) tc::mma_commit(tc::smem_u32(&fb.v_free[sl]));
+                    }
+                }
+                __syncwarp();
+            }
+            vc += w.nb;
         }
         if (elect_one()) tc::mma_commit(tc::smem_u32(&fb.fin[i]));
         __syncwarp();
         tc::mbar_wait(tc::smem_u32(&fb.fin[i]), 0, nullptr, 0);
-    } else if (warp >= 4 && warp < 12 && any) {
+    } else {
         // ---------------- softmax and epilogue: thread = query row ----------------
         const int i = (warp - 4) >> 2, quarter = warp & 3;
-        if (i < tiles) {
-            const int r = quarter * 32 + lane, j0 = r / a.G;     // row of the tile, token of the tile
-            const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-            const int tk = i * a.TQ + j0;                          // token of the CTA
-            const bool valid = r < a.G * a.TQ && tk < ntok;
+        const int r = quarter * 32 + lane, j0 = r / a.G, gh = r - j0 * a.G;   // row of the tile, its token and head
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        const uint32_t tS = tmem + lane_base + COL_S + i * 128, tO = tmem + lane_base + COL_O + i * 128;
+        const uint64_t sc2 = pack2(a.scale_log2, a.scale_log2);
+        const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
+        const int tk = i * a.TQ + j0;                              // token of the item
+        for (int it = 0, sc = 0;; ++it) {
+            // the item's description stays where it is until the end: registers are
+            // what this warp is short of
+            if (!wait_all(fb.work_full[it & 1], it >> 1, abort, a.err, PK_WORK)) break;
+            const Work &w = fb.work[it & 1];
+            if (w.end) break;
+            if (i >= w.tiles) {
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.work_free[it & 1]));
+                continue;
+            }
+            const bool valid = r < a.G * a.TQ && tk < w.ntok;
             int lim = -1;                                          // last key the row sees
             bool pad = !valid;
             if (valid) {
-                if (!a.prefix) lim = a.causal ? min(first_lim + tk, kend - 1) : kend - 1;
-                else if (__ldg(a.trow + tok0 + tk) >= 0) lim = min(__ldg(a.tpos + tok0 + tk), kend - 1);
+                if (!a.prefix) lim = a.causal ? min(w.first_lim + tk, w.kend - 1) : w.kend - 1;
+                else if (__ldg(a.trow + w.tok0 + tk) >= 0) lim = min(__ldg(a.tpos + w.tok0 + tk), w.kend - 1);
                 else pad = true;
             }
-            lim = pad ? 0x3fffffff : lim - kbeg;   // rows nobody reads need no mask
+            lim = pad ? 0x3fffffff : lim - w.kbeg;   // rows nobody reads need no mask
+            const int ns = w.ns;
             float m_used = -INFINITY, l = 0.f;
             bool ok = true;
-            const uint32_t tS = tmem + lane_base + COL_S + i * 128, tO = tmem + lane_base + COL_O + i * 128;
-            const uint64_t sc2 = pack2(a.scale_log2, a.scale_log2);
-            for (int n = 0; n < ns; ++n) {
-                const int b = n & 1;
-                ok = wait_all(fb.s_full[i][b], n >> 1, abort, a.err, PK_S);
+            for (int n = 0; n < ns; ++n, ++sc) {
+                const int b = sc & 1;
+                ok = wait_all(fb.s_full[i][b], sc >> 1, abort, a.err, PK_S);
                 if (!ok) break;
                 tc::fence_after_sync();
                 uint32_t v[SB];
@@ -465,7 +599,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 }
                 // a row whose reference moved scales its O once the last product is in
                 if (n && __any_sync(0xffffffffu, alpha != 1.f)) {
-                    ok = wait_all(fb.pv_done[i][b ^ 1], (n - 1) >> 1, abort, a.err, PK_PV);
+                    ok = wait_all(fb.pv_done[i][b ^ 1], (sc - 1) >> 1, abort, a.err, PK_PV);
                     if (!ok) break;
                     tc::fence_after_sync();
 #pragma unroll 1
@@ -494,59 +628,63 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.p_full[i][b]));
-                if (n == 0 && warp == 4 && lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.skew));
+                if (n == 0 && it == 0 && warp == 4 && lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.skew));
                 sum2[0] = add2(sum2[0], sum2[1]);
                 l = l * alpha + (lo2(sum2[0]) + hi2(sum2[0]));
             }
-            if (ok && nb) {
-                ok = wait_all(fb.pv_done[i][(ns - 1) & 1], (ns - 1) >> 1, abort, a.err, PK_PV) && !*abort;
-                ok = __all_sync(0xffffffffu, ok);
+            if (ok && ns) {
+                ok = wait_all(fb.pv_done[i][(sc - 1) & 1], (sc - 1) >> 1, abort, a.err, PK_PV);
+                ok = __all_sync(0xffffffffu, ok && !*abort);
                 tc::fence_after_sync();
             }
-            if (ok) {
-                const int gh = r - j0 * a.G;
-                const float inv = l != 0.f ? 1.f / l : 0.f;
-                const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
-                T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(tok0 + tk) * a.Hq + h * a.G + gh) * D;
-                const size_t prow = ((size_t)split * a.Hkv + h) * ((size_t)a.M * a.G) + (size_t)(tok0 + tk) * a.G + gh;
+            if (!ok) break;
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+            T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(w.tok0 + tk) * a.Hq + w.h * a.G + gh) * D;
+            const size_t prow = ((size_t)w.split * a.Hkv + w.h) * ((size_t)a.M * a.G) + (size_t)(w.tok0 + tk) * a.G + gh;
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.work_free[it & 1]));
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t acc[32];
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t acc[32];
+                __syncwarp();
+                if (ns) {
+                    tc::tmem_ld32(tO + c * 32, acc);
+                    tc::tmem_wait_ld();
+                }
+                if (ns && c + 1 == D / 32) {   // O may be written again
+                    tc::fence_before_sync();
                     __syncwarp();
-                    if (nb) {
-                        tc::tmem_ld32(tO + c * 32, acc);
-                        tc::tmem_wait_ld();
-                    }
-                    const bool live = nb && l != 0.f;
+                    if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.o_free[i]));
+                }
+                const bool live = ns && l != 0.f;
 #pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (!live) acc[x] = 0u;
-                    if (!pad && a.prefix) {
-                        float *p = a.o_part + prow * D + c * 32;
+                for (int x = 0; x < 32; ++x)
+                    if (!live) acc[x] = 0u;
+                if (!pad && a.prefix) {
+                    float *p = a.o_part + prow * D + c * 32;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) store32(p + x * 8, acc + x * 8);
-                    } else if (!pad) {
-                        uint32_t y[16];
+                    for (int x = 0; x < 4; ++x) store32(p + x * 8, acc + x * 8);
+                } else if (!pad) {
+                    uint32_t y[16];
 #pragma unroll
-                        for (int x = 0; x < 16; ++x)
-                            y[x] = Pk<T>::pack(__uint_as_float(acc[2 * x]) * inv, __uint_as_float(acc[2 * x + 1]) * inv);
-                        if (wide) {
-                            store32(dst + c * 32, y);
-                            store32(dst + c * 32 + 16, y + 8);
-                        } else {
+                    for (int x = 0; x < 16; ++x)
+                        y[x] = Pk<T>::pack(__uint_as_float(acc[2 * x]) * inv, __uint_as_float(acc[2 * x + 1]) * inv);
+                    if (wide) {
+                        store32(dst + c * 32, y);
+                        store32(dst + c * 32 + 16, y + 8);
+                    } else {
 #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                reinterpret_cast<uint4 *>(dst + c * 32)[x] = make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
-                        }
+                        for (int x = 0; x < 4; ++x)
+                            reinterpret_cast<uint4 *>(dst + c * 32)[x] = make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
                     }
                 }
-                if (a.prefix && !pad) *reinterpret_cast<float2 *>(a.ml_part + prow * 2) = make_float2(m_used, l);
             }
+            if (a.prefix && !pad) *reinterpret_cast<float2 *>(a.ml_part + prow * 2) = make_float2(m_used, l);
         }
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == 0 && nb) {
+    if (warp == 0) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, 512);
     }
