@@ -132,31 +132,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ uint64_t exp2_unit(uint64_t z) { return pack2(tc::ex2_approx(lo2(z)), tc::ex2_approx(hi2(z))); }
-
-// 2^z on the FMA pipe for finite z <= 8: z = n + r, n the nearest integer (taken
-// from the low bits of z + 1.5 * 2^23), 2^r by the polynomial 1 + r (c1 + ...) of
-// least relative error on [-1/2, 1/2] (1.0e-4 at degree 3, 2.8e-6 at degree 4,
-// fitted by reweighted least squares), n added to the exponent.  Below -126 the
-// result is 2^-126.
-template <int DEG>
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t z) {
-    z = pack2(fmaxf(lo2(z), -126.f), fmaxf(hi2(z), -126.f));
-    const uint64_t magic = pack2(12582912.f, 12582912.f), neg = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f);
-    const uint64_t t = add2(z, magic), r = fma2(add2(t, neg), minus, z), one = pack2(1.f, 1.f);
-    uint64_t p;
-    if (DEG == 3) {
-        p = fma2(r, pack2(0.055008933f, 0.055008933f), pack2(0.24221097f, 0.24221097f));
-        p = fma2(p, r, pack2(0.6932829f, 0.6932829f));
-    } else {
-        p = fma2(r, pack2(0.009582853f, 0.009582853f), pack2(0.055906426f, 0.055906426f));
-        p = fma2(p, r, pack2(0.24024099f, 0.24024099f));
-        p = fma2(p, r, pack2(0.69312418f, 0.69312418f));
-    }
-    p = fma2(p, r, one);
-    return pack2(__uint_as_float((uint32_t)p + ((uint32_t)t << 23)),
-                 __uint_as_float((uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23)));
-}
+__device__ __forceinline__ uint64_t exp2_2(uint64_t z) { return pack2(tc::ex2_approx(lo2(z)), tc::ex2_approx(hi2(z))); }
 
 // a whole 32-byte sector per thread: rows lie apart, so 16-byte stores would fill
 // every sector twice
@@ -169,7 +145,6 @@ template <typename T>
 struct Pk;
 template <>
 struct Pk<__half> {
-    static constexpr int POLY = 4, DEG = 4;   // pairs of 16 whose exponentials run on the FMA pipe
     static constexpr uint32_t fmt = 0;
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -178,7 +153,6 @@ struct Pk<__half> {
 };
 template <>
 struct Pk<__nv_bfloat16> {
-    static constexpr int POLY = 4, DEG = 3;
     static constexpr uint32_t fmt = (1u << 7) | (1u << 10);   // A and B bf16
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -619,7 +593,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
 #pragma unroll
                 for (int x = 0; x < SB / 2; ++x) {
                     const uint64_t z = fma2(pack2(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), sc2, nm2);
-                    const uint64_t e = exp2_unit(z);
+                    const uint64_t e = exp2_2(z);
                     sum2[x & 1] = add2(sum2[x & 1], e);
                     p[x] = Pk<T>::pack(lo2(e), hi2(e));
                 }
