@@ -254,11 +254,6 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     volatile int *abort = &fb.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // the kernel that follows a prefix pass starts on the SMs that this one leaves
-    // free, without waiting for it: so the pass's own predecessor must be done first
-    griddep_wait();
-    griddep_launch_dependents();
-
     if (threadIdx.x == 0) {
         for (int s = 0; s < KSLOTS; ++s) {
             tc::mbar_init(tc::smem_u32(&fb.k_full[s]), 1);
@@ -296,6 +291,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = fb.tmem;
+    // the kernel that follows a prefix pass starts on the SMs that this one leaves
+    // free, without waiting for it: so the pass's own predecessor must be done first
+    griddep_wait();
+    griddep_launch_dependents();
 
     // The next item of a reading warp (all but the producer): its number, then what
     // it is.  False at the end, or when the CTA has been given up.

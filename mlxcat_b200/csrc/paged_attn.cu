@@ -124,18 +124,25 @@ __device__ __forceinline__ float weight_of(float m, float l, float mx) {
 }
 
 // Shared memory: the warps' rings, the item's query rows, their limits.  The
-// merge of the warps reuses the rings.
+// merge of the warps has its own memory where two CTAs of an SM have room for it
+// (EARLY: the next piece's loads then run during the merge), else the rings'.
 template <int D, int NT>
 struct PagedShape {
     static constexpr int STAGE = 2 * TK * D * 2;            // K and V of one tile, bytes
     static constexpr int RING = PW * ST * STAGE;
     static constexpr int QR = NT * 8;                       // query rows of an item
     static constexpr int MT = D / 16, MTW = MT / PW;        // m tiles of O^T, and those a warp finishes
-    static constexpr int MERGE = PW * MT * NT * 512 + PW * QR * 8;
-    static constexpr int BODY = RING > MERGE ? RING : MERGE;
-    static constexpr int SMEM = BODY + QR * D * 2 + QR * 4;
+    static constexpr int FRAGS = PW * (PW - 1) * MTW * NT * 512;   // what the warps hand to one another
+    static constexpr int MERGE = FRAGS + PW * QR * 8;
+    static constexpr int TAIL = QR * D * 2 + QR * 4;
+    // the query operands stay in registers for two n8 tiles at most
+    static constexpr bool QREG = NT <= 2 || D == 64;
+    static constexpr bool EARLY = QREG && RING + MERGE + TAIL + 2304 <= (228 * 1024) / CTAS_PER_SM - 1024;
+    static constexpr int BODY = EARLY ? RING + MERGE : RING > MERGE ? RING : MERGE;
+    static constexpr int MERGE_AT = EARLY ? RING : 0;
+    static constexpr int SMEM = BODY + TAIL;
 };
-constexpr int MAX_GROUPS = 512;   // groups whose (row, last key) a CTA keeps
+constexpr int MAX_GROUPS = 256;   // groups whose (row, last key) a CTA keeps
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(PT, CTAS_PER_SM)
@@ -237,37 +244,103 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
     const uint32_t ring_a = tc::smem_u32(ring), qsm_a = tc::smem_u32(qsm);
     const int ch = lane % CH, r0 = lane / CH;
 
-    for (int64_t u = u0; u < u1;) {
-        while (u >= ubase + (int64_t)gu * per_group) {
-            ubase += (int64_t)gu * per_group;
-            gi = group(++grp);
-            gu = units_of(gi);
+    // A piece: this CTA's part of an item.
+    struct Piece {
+        int64_t ib;             // the item's first unit
+        size_t item;
+        const T *kb, *vb;
+        const int32_t *table;
+        int gu, h, qt, t0, nq, kend, ua, steps, kfirst;
+        bool whole;
+    };
+    int64_t u = u0;
+    auto next_piece = [&](Piece &p) -> bool {
+        while (u < u1) {
+            while (u >= ubase + (int64_t)gu * per_group) {
+                ubase += (int64_t)gu * per_group;
+                gi = group(++grp);
+                gu = units_of(gi);
+            }
+            const int x = (int)((u - ubase) / gu);                 // item of the group
+            p.ib = ubase + (int64_t)x * gu;
+            const int va = (int)(u - p.ib), vend = (int)min((int64_t)gu, u1 - p.ib);
+            u = p.ib + vend;
+            p.ua = max(va - LEAD, 0);
+            p.steps = vend - LEAD - p.ua;                          // units of keys
+            if (p.steps <= 0) continue;                            // leading units only
+            p.whole = p.ua == 0 && vend == gu;
+            p.gu = gu;
+            p.h = x / qts;
+            p.qt = x - p.h * qts;
+            p.t0 = grp * a.qg;
+            p.nq = min(S::QR, min(a.qg, a.M - p.t0) * G - p.qt * S::QR);   // may be <= 0 in a last, short group
+            p.item = (size_t)grp * per_group + x;
+            p.kend = gi.kend;
+            p.kfirst = key_begin + p.ua * UNIT + warp * TK;        // key 0 of step 0 (fits: below the table's capacity + UNIT)
+            p.kb = reinterpret_cast<const T *>(kv.k) + (int64_t)p.h * kv.head_stride;
+            p.vb = reinterpret_cast<const T *>(kv.v) + (int64_t)p.h * kv.head_stride;
+            p.table = kv.table + (size_t)gi.row * kv.max_pages;
+            return true;
         }
-        const int x = (int)((u - ubase) / gu);                 // item of the group
-        const int64_t ib = ubase + (int64_t)x * gu;            // its first unit
-        const int va = (int)(u - ib), vend = (int)min((int64_t)gu, u1 - ib);   // this CTA's part of it
-        u = ib + vend;
-        const int ua = max(va - LEAD, 0), ub = vend - LEAD;                       // units of keys
-        if (ub <= ua) continue;                                                 // leading units only
-        const bool whole = ua == 0 && vend == gu;
-        const int h = x / qts, qt = x - h * qts;
-        const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
-        const int nq = min(S::QR, ntok * G - qt * S::QR);      // may be <= 0 in a last, short group
-        const size_t item = (size_t)grp * per_group + x;
-
-        // ---- the item's query rows and key limits into shared memory
+        return false;
+    };
+    const int pmask = (1 << kv.page_shift) - 1;
+    int pid[2] = {-1, -1};       // lane l: pages of the two 8-key halves of step (32 batch + l)
+    auto stage = [&](const Piece &p, int s) {
+        if ((s & 31) == 0) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int64_t key = (int64_t)p.kfirst + (int64_t)(s + lane) * UNIT + 8 * e;
+                int id = -1;
+                if (s + lane < p.steps && key < p.kend) {
+                    id = __ldg(p.table + (key >> kv.page_shift));
+                    if (id < 0 || id >= kv.n_pages) {
+                        id = -1;
+                        if (a.err) atomicExch(a.err, PE_PAGE);
+                    }
+                }
+                pid[e] = id;
+            }
+        }
+        const int p0 = __shfl_sync(0xffffffffu, pid[0], s & 31), p1 = __shfl_sync(0xffffffffu, pid[1], s & 31);
+        const uint32_t dst = ring_a + (uint32_t)(s % ST) * S::STAGE;
+        const int key0 = p.kfirst + s * UNIT;
+#pragma unroll
+        for (int i = 0; i < TK / RPI; ++i) {
+            const int r = r0 + i * RPI, key = key0 + r;
+            const int id = r < 8 ? p0 : p1;
+            const bool ok = key < p.kend && id >= 0;
+            const int64_t off = ok ? (int64_t)id * kv.page_stride + (int64_t)(key & pmask) * kv.token_stride + ch * 8 : 0;
+            const uint32_t so = dst + (uint32_t)(r * D * 2 + ((ch ^ (r & 7)) << 4));
+            cpa16(so, p.kb + off, ok ? 16 : 0);
+            cpa16(so + TK * D * 2, p.vb + off, ok ? 16 : 0);
+        }
+    };
+    // the piece's query rows and key limits into shared memory, its first tiles into the ring
+    auto begin = [&](const Piece &p) {
         for (int w = threadIdx.x; w < S::QR * CH; w += PT) {
-            const int r = w / CH, c = w % CH, rr = qt * S::QR + r, j = div_g(rr);
-            const bool ok = r < nq;
-            const T *src = reinterpret_cast<const T *>(a.q) + ((size_t)(t0 + (ok ? j : 0)) * Hq + h * G + (ok ? rr - j * G : 0)) * D + c * 8;
+            const int r = w / CH, c = w % CH, rr = p.qt * S::QR + r, j = div_g(rr);
+            const bool ok = r < p.nq;
+            const T *src = reinterpret_cast<const T *>(a.q) + ((size_t)(p.t0 + (ok ? j : 0)) * Hq + p.h * G + (ok ? rr - j * G : 0)) * D + c * 8;
             cpa16(qsm_a + (uint32_t)(r * D * 2 + ((c ^ (r & 7)) << 4)), src, ok ? 16 : 0);
         }
         if (threadIdx.x < S::QR) {
-            const int r = threadIdx.x, m = t0 + div_g(qt * S::QR + r);
+            const int r = threadIdx.x, m = p.t0 + div_g(p.qt * S::QR + r);
             // rows nobody reads see everything: they need no mask
-            lim_s[r] = r < nq && __ldg(a.trow + m) >= 0 ? __ldg(a.tpos + m) : 0x7fffffff;
+            lim_s[r] = r < p.nq && __ldg(a.trow + m) >= 0 ? __ldg(a.tpos + m) : 0x7fffffff;
         }
+#pragma unroll
+        for (int s = 0; s < ST - 1; ++s) {
+            if (s < p.steps) stage(p, s);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        }
+    };
 
+    Piece pc, pn;
+    bool have = next_piece(pc);
+    if (have) begin(pc);
+    while (have) {
+        const int qt = pc.qt, h = pc.h, t0 = pc.t0, nq = pc.nq;
         float o[D / 16][NT][4], ls[NT][4], mr[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -278,50 +351,6 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[mt][nt][i] = 0.f;
-        }
-
-        const int steps = ub - ua;
-        const int kfirst = key_begin + ua * UNIT + warp * TK;   // key 0 of step 0 (fits: below the table's capacity + UNIT)
-        const T *kb = reinterpret_cast<const T *>(kv.k) + (int64_t)h * kv.head_stride;
-        const T *vb = reinterpret_cast<const T *>(kv.v) + (int64_t)h * kv.head_stride;
-        const int32_t *table = kv.table + (size_t)gi.row * kv.max_pages;
-        const int pmask = (1 << kv.page_shift) - 1;
-        int pid[2] = {-1, -1};       // lane l: pages of the two 8-key halves of step (32 batch + l)
-        auto lookup = [&](int step0) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int64_t key = (int64_t)kfirst + (int64_t)(step0 + lane) * UNIT + 8 * e;
-                int p = -1;
-                if (step0 + lane < steps && key < gi.kend) {
-                    p = __ldg(table + (key >> kv.page_shift));
-                    if (p < 0 || p >= kv.n_pages) {
-                        p = -1;
-                        if (a.err) atomicExch(a.err, PE_PAGE);
-                    }
-                }
-                pid[e] = p;
-            }
-        };
-        auto stage = [&](int s) {
-            if ((s & 31) == 0) lookup(s);
-            const int p0 = __shfl_sync(0xffffffffu, pid[0], s & 31), p1 = __shfl_sync(0xffffffffu, pid[1], s & 31);
-            const uint32_t dst = ring_a + (uint32_t)(s % ST) * S::STAGE;
-            const int key0 = kfirst + s * UNIT;
-#pragma unroll
-            for (int i = 0; i < TK / RPI; ++i) {
-                const int r = r0 + i * RPI, key = key0 + r;
-                const int p = r < 8 ? p0 : p1;
-                const bool ok = key < gi.kend && p >= 0;
-                const int64_t off = ok ? (int64_t)p * kv.page_stride + (int64_t)(key & pmask) * kv.token_stride + ch * 8 : 0;
-                const uint32_t so = dst + (uint32_t)(r * D * 2 + ((ch ^ (r & 7)) << 4));
-                cpa16(so, kb + off, ok ? 16 : 0);
-                cpa16(so + TK * D * 2, vb + off, ok ? 16 : 0);
-            }
-        };
-#pragma unroll
-        for (int s = 0; s < ST - 1; ++s) {
-            if (s < steps) stage(s);
-            asm volatile("cp.async.commit_group;\n" ::: "memory");
         }
         asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 2) : "memory");   // the queries came with the first stage
         __syncthreads();
@@ -334,20 +363,21 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             const int r = nt * 8 + (lane & 7);
 #pragma unroll
             for (int ks = 0; ks < D / 16; ks += 2)
-                ldm4(&qf[nt][ks][0], qsm_a + (uint32_t)(r * D * 2 + (((ks * 2 + (lane >> 3)) ^ (r & 7)) << 4)));
+                if (S::QREG) ldm4(&qf[nt][ks][0], qsm_a + (uint32_t)(r * D * 2 + (((ks * 2 + (lane >> 3)) ^ (r & 7)) << 4)));
             lim[nt][0] = lim_s[nt * 8 + 2 * t];
             lim[nt][1] = lim_s[nt * 8 + 2 * t + 1];
             lim_min = min(lim_min, min(lim[nt][0], lim[nt][1]));
         }
         lim_min = __reduce_min_sync(0xffffffffu, lim_min);
-        for (int s = 0; s < steps; ++s) {
+        if (S::EARLY) __syncthreads();   // the next piece's may come in
+        for (int s = 0; s < pc.steps; ++s) {
             __syncwarp();            // every lane has read the stage that is filled now
-            if (s + ST - 1 < steps) stage(s + ST - 1);
+            if (s + ST - 1 < pc.steps) stage(pc, s + ST - 1);
             asm volatile("cp.async.commit_group;\n" ::: "memory");
             asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 1) : "memory");
             __syncwarp();
-            const int key0 = kfirst + s * UNIT;
-            if (key0 >= gi.kend) continue;   // no key of this tile (a last unit)
+            const int key0 = pc.kfirst + s * UNIT;
+            if (key0 >= pc.kend) continue;   // no key of this tile (a last unit)
             const uint32_t ka = ring_a + (uint32_t)(s % ST) * S::STAGE, va = ka + TK * D * 2;
             float sc[NT][4];
 #pragma unroll
@@ -355,20 +385,32 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             {
                 const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    uint32_t f[4];
-                    ldm4(f, ka + (uint32_t)(r * D * 2 + (((ks * 2 + (lane >> 4)) ^ (r & 7)) << 4)));
+                for (int ks = 0; ks < D / 16; ks += 2) {
+                    uint32_t f[2][4];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) Half2<T>::mma(sc[nt], f, qf[nt][ks][0], qf[nt][ks][1]);
+                    for (int e = 0; e < 2; ++e)
+                        ldm4(f[e], ka + (uint32_t)(r * D * 2 + ((((ks + e) * 2 + (lane >> 4)) ^ (r & 7)) << 4)));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        uint32_t q[4];
+                        if (S::QREG) {
+                            q[0] = qf[nt][ks][0]; q[1] = qf[nt][ks][1]; q[2] = qf[nt][ks + 1][0]; q[3] = qf[nt][ks + 1][1];
+                        } else {
+                            const int qr = nt * 8 + (lane & 7);
+                            ldm4(q, qsm_a + (uint32_t)(qr * D * 2 + (((ks * 2 + (lane >> 3)) ^ (qr & 7)) << 4)));
+                        }
+                        Half2<T>::mma(sc[nt], f[0], q[0], q[1]);
+                        Half2<T>::mma(sc[nt], f[1], q[2], q[3]);
+                    }
                 }
             }
-            if (key0 + TK - 1 > lim_min || key0 + TK > gi.kend) {
+            if (key0 + TK - 1 > lim_min || key0 + TK > pc.kend) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = key0 + g + (i >> 1) * 8;
-                        if (key > lim[nt][i & 1] || key >= gi.kend) sc[nt][i] = -INFINITY;
+                        if (key > lim[nt][i & 1] || key >= pc.kend) sc[nt][i] = -INFINITY;
                     }
             }
             bool raise = false;
@@ -421,27 +463,36 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             }
         }
 
-        // ---- merge the warps' partials through the rings' memory: every warp
-        // finishes MTW m tiles of O^T, as accumulator fragments [warp][m tile][nt][lane]
-        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-        __syncthreads();
-        float4 *of = reinterpret_cast<float4 *>(psm);
-        float2 *mls = reinterpret_cast<float2 *>(psm + PW * S::MT * NT * 512);   // [warp][QR] (max, sum)
+        // ---- merge the warps' partials: every warp finishes MTW m tiles of O^T and
+        // gets the others' accumulator fragments of them ([from][to][m tile][nt][lane])
+        const bool more = next_piece(pn);
+        if (S::EARLY) {
+            __syncwarp();   // every lane is through with the ring
+            if (more) begin(pn);
+        } else {
+            asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+            __syncthreads();
+        }
+        float4 *of = reinterpret_cast<float4 *>(psm + S::MERGE_AT);
+        float2 *mls = reinterpret_cast<float2 *>(psm + S::MERGE_AT + S::FRAGS);   // [warp][QR] (max, sum)
+        auto frag = [&](int src, int mt, int nt) {
+            const int to = mt / S::MTW;
+            return (((src * (PW - 1) + to - (to > src)) * S::MTW + mt % S::MTW) * NT + nt) * 32 + lane;
+        };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int mt = 0; mt < S::MT; ++mt)
-                if (mt / S::MTW != warp)
-                    of[((warp * S::MT + mt) * NT + nt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
+                if (mt / S::MTW != warp) of[frag(warp, mt, nt)] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
             if (g == 0) {
                 mls[warp * S::QR + nt * 8 + 2 * t] = make_float2(mr[nt][0], ls[nt][0]);
                 mls[warp * S::QR + nt * 8 + 2 * t + 1] = make_float2(mr[nt][1], ls[nt][1]);
             }
         }
         __syncthreads();
-        const bool direct = whole && !force_partial;
+        const bool direct = pc.whole && !force_partial;
         // slots in order of (item, CTA): unique, since a piece starts a new item or a new CTA
-        const size_t slot = item + blockIdx.x;
+        const size_t slot = pc.item + blockIdx.x;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float f[2][PW], l[2], mx[2];
@@ -478,7 +529,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
 #pragma unroll
                 for (int i = 0; i < PW; ++i) {
                     const float4 z = i == warp ? make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3])
-                                               : of[((i * S::MT + mt) * NT + nt) * 32 + lane];
+                                               : of[frag(i, mt, nt)];
                     y[0] += f[0][i] * z.x; y[1] += f[1][i] * z.y; y[2] += f[0][i] * z.z; y[3] += f[1][i] * z.w;
                 }
                 if (direct) {
@@ -495,12 +546,15 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
                 }
             }
         }
-        // the CTA that holds an item's first unit says where its pieces are
-        if (ua == 0 && threadIdx.x == 0) {
-            const int last = (int)(((ib + gu) * C - 1) / U);
-            meta[item] = direct ? make_int2(0, -2) : make_int2(blockIdx.x, last);
+        // the CTA that holds an item's first keys says where its pieces are
+        if (pc.ua == 0 && threadIdx.x == 0) {
+            const int last = (int)(((pc.ib + pc.gu) * C - 1) / U);
+            meta[pc.item] = direct ? make_int2(0, -2) : make_int2(blockIdx.x, last);
         }
-        __syncthreads();   // the ring is filled again
+        __syncthreads();   // the merge's memory is used again
+        if (!S::EARLY && more) begin(pn);
+        pc = pn;
+        have = more;
     }
     if (force_partial) griddep_wait();
 }
@@ -522,7 +576,7 @@ attn_join(const PagedKV kv, const PagedQuery a, int QR, const float *__restrict_
     const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
     const int nq = min(QR, ntok * G - qt * QR);
     const int n_own = mt.y >= 0 ? mt.y - mt.x + 1 : 0, n = n_own + pre.splits;
-    constexpr int PB = 6;   // pieces whose loads are in flight together
+    constexpr int PB = 8;   // pieces whose loads are in flight together
     for (int w = threadIdx.x; w < nq * (D / 8); w += blockDim.x) {
         const int r = w / (D / 8), d = (w % (D / 8)) * 8;
         const int rr = qt * QR + r, m = t0 + rr / G;
@@ -622,7 +676,10 @@ cudaError_t run(const PagedKV &kv, const PagedQuery &q, int key_begin, const Pre
                 int sm_count, cudaStream_t st) {
     const int G = q.n_heads / kv.n_kv, NT = paged_nt(q.qg, G);
     const Scratch s = scratch_of(q.M, q.qg, q.n_heads, kv.n_kv, D, sm_count);
-    const int grid = sm_count * CTAS_PER_SM;
+    // no more CTAs than the table can hold units for: behind a prefix pass the ones
+    // without a free SM would only start when the pass ends
+    const int64_t cap = std::max(0, paged_capacity(kv) - key_begin);
+    const int grid = (int)std::min<int64_t>((int64_t)sm_count * CTAS_PER_SM, (int64_t)s.items * ((cap + UNIT - 1) / UNIT + LEAD));
     const bool partial = pre.splits > 0;
     cudaError_t e;
     switch (NT) {
