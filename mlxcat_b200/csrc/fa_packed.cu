@@ -185,7 +185,7 @@ __device__ __forceinline__ bool next_item(uint32_t response, int *id) {
     return got != 0;
 }
 
-// Item `id` of the grid; ntok <= 0: none there.
+// Item `id` of the grid, for a whole warp; ntok <= 0: none there.
 __device__ __forceinline__ Work work_of(const Args &a, int id) {
     Work w = {};
     w.h = id % a.Hkv;
@@ -194,16 +194,31 @@ __device__ __forceinline__ Work work_of(const Args &a, int id) {
         // sequence s owns tile numbers from cu_q[s] / (2 TQ) + s on: one more than
         // its tokens need at most, so the map needs no prefix sum
         const int tile = gridDim.x / a.Hkv - 1 - x;   // the last tiles see most keys: first
-        int lo = 0, hi = a.n_seq - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (__ldg(a.cu_q + mid) / (2 * a.TQ) + mid <= tile) lo = mid;
-            else hi = mid - 1;
+        // the last sequence that starts at or before it, 32 probes at a time; the last
+        // round's loads bring the sequence's bounds along
+        const int lane = threadIdx.x & 31;
+        int lo = 0, n = a.n_seq;
+        while (n > 32) {
+            const int step = (n + 31) / 32, at = lo + lane * step;
+            const bool in = lane * step < n && __ldg(a.cu_q + at) / (2 * a.TQ) + at <= tile;
+            const int k = max(__popc(__ballot_sync(0xffffffffu, in)) - 1, 0);
+            lo += k * step;
+            n = min(step, n - k * step);
         }
+        int c[4] = {0, 0, 0, 0};
+        if (lane < n) {
+            c[0] = __ldg(a.cu_q + lo + lane);
+            c[1] = __ldg(a.cu_q + lo + lane + 1);
+            c[2] = __ldg(a.cu_k + lo + lane);
+            c[3] = __ldg(a.cu_k + lo + lane + 1);
+        }
+        const int k = max(__popc(__ballot_sync(0xffffffffu, lane < n && c[0] / (2 * a.TQ) + lo + lane <= tile)) - 1, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = __shfl_sync(0xffffffffu, c[i], k);
         // offsets outside the buffers are cut to them
-        const int q0 = min(max(__ldg(a.cu_q + lo), 0), a.Tq), q1 = min(max(__ldg(a.cu_q + lo + 1), q0), a.Tq);
-        const int k0 = min(max(__ldg(a.cu_k + lo), 0), a.Tk), k1 = min(max(__ldg(a.cu_k + lo + 1), k0), a.Tk);
-        const int at = (tile - (__ldg(a.cu_q + lo) / (2 * a.TQ) + lo)) * 2 * a.TQ;   // token of the sequence
+        const int q0 = min(max(c[0], 0), a.Tq), q1 = min(max(c[1], q0), a.Tq);
+        const int k0 = min(max(c[2], 0), a.Tk), k1 = min(max(c[3], k0), a.Tk);
+        const int at = (tile - (c[0] / (2 * a.TQ) + lo + k)) * 2 * a.TQ;   // token of the sequence
         if (at >= 0 && at < q1 - q0) {
             w.tok0 = q0 + at;
             w.ntok = min(2 * a.TQ, q1 - w.tok0);

@@ -43,6 +43,7 @@ constexpr int CTAS_PER_SM = 2;
 // loads, merge: 5,500 cycles) as three units of keys: its stretch has that many
 // units without keys in front, so that CTAs of many short items are not the last.
 constexpr int LEAD = 3;
+constexpr int ONE_CLUSTER = 8, CLUSTER_UNITS = 8;   // CTAs of a small call's cluster, units each at most
 
 template <typename T>
 struct Half2;
@@ -144,10 +145,90 @@ struct PagedShape {
 };
 constexpr int MAX_GROUPS = 256;   // groups whose (row, last key) a CTA keeps
 
+// Merge an item's pieces (and, after a shared prefix, the prefix's splits):
+// thread = 8 features of a query row; pieces in order.
+template <typename T, int D>
+__device__ __forceinline__ void join_item(const PagedKV &kv, const PagedQuery &a, int QR, size_t item,
+                                          const float *o_part, const float *ml_part, int2 mt, const PrefixPartials &pre) {
+    const int Hq = a.n_heads, G = Hq / kv.n_kv;
+    const int qts = (a.qg * G + QR - 1) / QR, per_group = kv.n_kv * qts;
+    const int grp = (int)(item / per_group), x = (int)(item % per_group), h = x / qts, qt = x - h * qts;
+    if (mt.y < 0 && pre.splits == 0) return;   // written already
+    const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
+    const int nq = min(QR, ntok * G - qt * QR);
+    const int n_own = mt.y >= 0 ? mt.y - mt.x + 1 : 0, n = n_own + pre.splits;
+    constexpr int PB = 8;   // pieces whose loads are in flight together
+    for (int w = threadIdx.x; w < nq * (D / 8); w += blockDim.x) {
+        const int r = w / (D / 8), d = (w % (D / 8)) * 8;
+        const int rr = qt * QR + r, m = t0 + rr / G;
+        if (__ldg(a.trow + m) < 0) continue;
+        float acc[8], l = 0.f, mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+        for (int p0 = 0; p0 < n; p0 += PB) {
+            float2 ml[PB];
+            float4 va[PB], vb[PB];
+#pragma unroll
+            for (int k = 0; k < PB; ++k) {
+                ml[k] = make_float2(-INFINITY, 0.f);
+                va[k] = vb[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int p = p0 + k;
+                if (p < n) {
+                    size_t at;
+                    const float *os, *ms;
+                    if (p < n_own) {
+                        at = (item + mt.x + p) * QR + r;
+                        os = o_part; ms = ml_part;
+                    } else {
+                        at = ((size_t)(p - n_own) * kv.n_kv + h) * ((size_t)a.M * G) + (size_t)t0 * G + rr;
+                        os = pre.o; ms = pre.ml;
+                    }
+                    ml[k] = *reinterpret_cast<const float2 *>(ms + at * 2);
+                    va[k] = *reinterpret_cast<const float4 *>(os + at * D + d);
+                    vb[k] = *reinterpret_cast<const float4 *>(os + at * D + d + 4);
+                }
+            }
+            float mb = mx;
+#pragma unroll
+            for (int k = 0; k < PB; ++k) mb = fmaxf(mb, ml[k].x);
+            if (mx != -INFINITY && mx != mb) {
+                const float f = tc::ex2_approx(mx - mb);
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] *= f;
+            }
+            mx = mb;
+#pragma unroll
+            for (int k = 0; k < PB; ++k) {
+                const float f = weight_of(ml[k].x, ml[k].y, mb);
+                l += f * ml[k].y;
+                acc[0] += f * va[k].x; acc[1] += f * va[k].y; acc[2] += f * va[k].z; acc[3] += f * va[k].w;
+                acc[4] += f * vb[k].x; acc[5] += f * vb[k].y; acc[6] += f * vb[k].z; acc[7] += f * vb[k].w;
+            }
+        }
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        uint4 y;
+        y.x = Half2<T>::pack(acc[0] * inv, acc[1] * inv);
+        y.y = Half2<T>::pack(acc[2] * inv, acc[3] * inv);
+        y.z = Half2<T>::pack(acc[4] * inv, acc[5] * inv);
+        y.w = Half2<T>::pack(acc[6] * inv, acc[7] * inv);
+        *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr % G) * D + d) = y;
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+attn_join(const PagedKV kv, const PagedQuery a, int QR, const float *__restrict__ o_part,
+          const float *__restrict__ ml_part, const int2 *__restrict__ meta, const PrefixPartials pre) {
+    griddep_launch_dependents();
+    griddep_wait();
+    join_item<T, D>(kv, a, QR, blockIdx.x, o_part, ml_part, meta[blockIdx.x], pre);
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(PT, CTAS_PER_SM)
-paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force_partial, float *__restrict__ o_part,
-                  float *__restrict__ ml_part, int2 *__restrict__ meta) {
+paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force_partial, float *o_part, float *ml_part,
+                  int2 *meta, const PrefixPartials pre, int one_cluster, int items) {
     using S = PagedShape<D, NT>;
     constexpr int CH = D / 8;            // 16-byte chunks per key
     constexpr int RPI = 32 / CH;         // keys per load instruction of a warp
@@ -231,13 +312,9 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             for (int x = lane; x < Hq * D / 8; x += 32) dst[x] = make_uint4(0, 0, 0, 0);
         }
     }
-    if (u1 <= u0) {
-        if (force_partial) griddep_wait();
-        return;
-    }
-
-    int grp = (int)start_s[0];
-    int64_t ubase = start_s[1];          // units before this group
+    const bool work = u1 > u0;
+    int grp = work ? (int)start_s[0] : 0;
+    int64_t ubase = work ? start_s[1] : 0;   // units before this group
     Group gi = group(grp);
     int gu = units_of(gi);               // units per item
     unsigned char *ring = psm + warp * (ST * S::STAGE);
@@ -557,81 +634,11 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         have = more;
     }
     if (force_partial) griddep_wait();
-}
-
-// Merge an item's pieces (and, after a shared prefix, the prefix's splits):
-// thread = 8 features of a query row; pieces in order.
-template <typename T, int D>
-__global__ void __launch_bounds__(256)
-attn_join(const PagedKV kv, const PagedQuery a, int QR, const float *__restrict__ o_part,
-          const float *__restrict__ ml_part, const int2 *__restrict__ meta, const PrefixPartials pre) {
-    griddep_launch_dependents();
-    griddep_wait();
-    const int Hq = a.n_heads, G = Hq / kv.n_kv;
-    const int qts = (a.qg * G + QR - 1) / QR, per_group = kv.n_kv * qts;
-    const size_t item = blockIdx.x;
-    const int grp = (int)(item / per_group), x = (int)(item % per_group), h = x / qts, qt = x - h * qts;
-    const int2 mt = meta[item];
-    if (mt.y < 0 && pre.splits == 0) return;   // written already
-    const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
-    const int nq = min(QR, ntok * G - qt * QR);
-    const int n_own = mt.y >= 0 ? mt.y - mt.x + 1 : 0, n = n_own + pre.splits;
-    constexpr int PB = 8;   // pieces whose loads are in flight together
-    for (int w = threadIdx.x; w < nq * (D / 8); w += blockDim.x) {
-        const int r = w / (D / 8), d = (w % (D / 8)) * 8;
-        const int rr = qt * QR + r, m = t0 + rr / G;
-        if (__ldg(a.trow + m) < 0) continue;
-        float acc[8], l = 0.f, mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-        for (int p0 = 0; p0 < n; p0 += PB) {
-            float2 ml[PB];
-            float4 va[PB], vb[PB];
-#pragma unroll
-            for (int k = 0; k < PB; ++k) {
-                ml[k] = make_float2(-INFINITY, 0.f);
-                va[k] = vb[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                const int p = p0 + k;
-                if (p < n) {
-                    size_t at;
-                    const float *os, *ms;
-                    if (p < n_own) {
-                        at = (item + mt.x + p) * QR + r;
-                        os = o_part; ms = ml_part;
-                    } else {
-                        at = ((size_t)(p - n_own) * kv.n_kv + h) * ((size_t)a.M * G) + (size_t)t0 * G + rr;
-                        os = pre.o; ms = pre.ml;
-                    }
-                    ml[k] = *reinterpret_cast<const float2 *>(ms + at * 2);
-                    va[k] = *reinterpret_cast<const float4 *>(os + at * D + d);
-                    vb[k] = *reinterpret_cast<const float4 *>(os + at * D + d + 4);
-                }
-            }
-            float mb = mx;
-#pragma unroll
-            for (int k = 0; k < PB; ++k) mb = fmaxf(mb, ml[k].x);
-            if (mx != -INFINITY && mx != mb) {
-                const float f = tc::ex2_approx(mx - mb);
-                l *= f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] *= f;
-            }
-            mx = mb;
-#pragma unroll
-            for (int k = 0; k < PB; ++k) {
-                const float f = weight_of(ml[k].x, ml[k].y, mb);
-                l += f * ml[k].y;
-                acc[0] += f * va[k].x; acc[1] += f * va[k].y; acc[2] += f * va[k].z; acc[3] += f * va[k].w;
-                acc[4] += f * vb[k].x; acc[5] += f * vb[k].y; acc[6] += f * vb[k].z; acc[7] += f * vb[k].w;
-            }
-        }
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        uint4 y;
-        y.x = Half2<T>::pack(acc[0] * inv, acc[1] * inv);
-        y.y = Half2<T>::pack(acc[2] * inv, acc[3] * inv);
-        y.z = Half2<T>::pack(acc[4] * inv, acc[5] * inv);
-        y.w = Half2<T>::pack(acc[6] * inv, acc[7] * inv);
-        *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr % G) * D + d) = y;
+    if (one_cluster) {
+        // a call of few units is one cluster: it joins its pieces itself, behind a
+        // barrier that also orders their stores
+        asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        for (size_t i = blockIdx.x; i < (size_t)items; i += gridDim.x) join_item<T, D>(kv, a, S::QR, i, o_part, ml_part, meta[i], pre);
     }
 }
 
@@ -654,8 +661,8 @@ Scratch scratch_of(int M, int qg, int n_heads, int n_kv, int D, int sm_count) {
 }
 
 template <typename T, int D, int NT>
-cudaError_t launch_main(const PagedKV &kv, const PagedQuery &q, int key_begin, bool partial, const Scratch &s, char *ws,
-                        int grid, cudaStream_t st) {
+cudaError_t launch_main(const PagedKV &kv, const PagedQuery &q, int key_begin, const PrefixPartials &pre, const Scratch &s,
+                        char *ws, int grid, bool cluster, cudaStream_t st) {
     using P = PagedShape<D, NT>;
     static bool attr[64] = {};
     int dev = 0;
@@ -666,9 +673,22 @@ cudaError_t launch_main(const PagedKV &kv, const PagedQuery &q, int key_begin, b
         if (e != cudaSuccess) return e;
         attr[dev & 63] = true;
     }
-    return launch_pdl(paged_attn_kernel<T, D, NT>, dim3(grid), dim3(PT), (size_t)P::SMEM, st, kv, q, key_begin,
-                      partial ? 1 : 0, reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + s.ml_at),
-                      reinterpret_cast<int2 *>(ws + s.meta_at));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(PT);
+    cfg.dynamicSmemBytes = P::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = grid;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, paged_attn_kernel<T, D, NT>, kv, q, key_begin, pre.splits > 0 ? 1 : 0,
+                              reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + s.ml_at),
+                              reinterpret_cast<int2 *>(ws + s.meta_at), pre, cluster ? 1 : 0, (int)s.items);
 }
 
 template <typename T, int D>
@@ -679,16 +699,18 @@ cudaError_t run(const PagedKV &kv, const PagedQuery &q, int key_begin, const Pre
     // no more CTAs than the table can hold units for: behind a prefix pass the ones
     // without a free SM would only start when the pass ends
     const int64_t cap = std::max(0, paged_capacity(kv) - key_begin);
-    const int grid = (int)std::min<int64_t>((int64_t)sm_count * CTAS_PER_SM, (int64_t)s.items * ((cap + UNIT - 1) / UNIT + LEAD));
-    const bool partial = pre.splits > 0;
+    const int64_t units = (int64_t)s.items * ((cap + UNIT - 1) / UNIT + LEAD);
+    // few units: one cluster that joins its own pieces, no second kernel
+    const bool cluster = units <= ONE_CLUSTER * CLUSTER_UNITS;
+    const int grid = (int)std::min<int64_t>(cluster ? ONE_CLUSTER : (int64_t)sm_count * CTAS_PER_SM, units);
     cudaError_t e;
     switch (NT) {
-        case 1: e = launch_main<T, D, 1>(kv, q, key_begin, partial, s, ws, grid, st); break;
-        case 2: e = launch_main<T, D, 2>(kv, q, key_begin, partial, s, ws, grid, st); break;
-        case 3: e = launch_main<T, D, 3>(kv, q, key_begin, partial, s, ws, grid, st); break;
-        default: e = launch_main<T, D, 4>(kv, q, key_begin, partial, s, ws, grid, st); break;
+        case 1: e = launch_main<T, D, 1>(kv, q, key_begin, pre, s, ws, grid, cluster, st); break;
+        case 2: e = launch_main<T, D, 2>(kv, q, key_begin, pre, s, ws, grid, cluster, st); break;
+        case 3: e = launch_main<T, D, 3>(kv, q, key_begin, pre, s, ws, grid, cluster, st); break;
+        default: e = launch_main<T, D, 4>(kv, q, key_begin, pre, s, ws, grid, cluster, st); break;
     }
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || cluster) return e;
     const int threads = std::min(256, (NT * 8 * (D / 8) + 31) / 32 * 32);
     return launch_pdl(attn_join<T, D>, dim3((unsigned)s.items), dim3(threads), 0, st, kv, q, NT * 8,
                       (const float *)ws, (const float *)(ws + s.ml_at), (const int2 *)(ws + s.meta_at), pre);
