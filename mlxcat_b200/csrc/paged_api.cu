@@ -240,6 +240,14 @@ int mlxcat_op_shared_prefix_attention(const mlxcat_paged_kv *c, int32_t prefix_l
     if (sms <= 0) return op_error(MLXCAT_E_CUDA, "paged attention: no CUDA device");
     PrefixPartials pre;
     const cudaStream_t st = (cudaStream_t)stream;
+    // What the rows would read of the prefix one by one.  As long as that is about
+    // what L2 holds, reading it per row is the shorter way, since the pass over the
+    // shared keys and the join of its partials cost 12 us by themselves: 8 KV heads
+    // of 128, 32 rows, 256 keys (34 MB) 15 us per row against 22 us shared, 1,024
+    // keys (134 MB) 23 against 23, 64 rows and 1,024 keys (268 MB) 38 against 31,
+    // 4,096 keys (1.1 GB) 106 against 37.
+    const int64_t apart = (int64_t)((M + pq.qg - 1) / pq.qg) * prefix_len * kv.n_kv * kv.D * 4;
+    if (apart <= ((int64_t)128 << 20)) prefix_len = 0;
     if (prefix_len) {
         const PrefixLayout l = prefix_layout(M, n_heads, kv.n_kv, kv.D, prefix_len);
         char *at = static_cast<char *>(workspace) + own;

@@ -145,84 +145,120 @@ struct PagedShape {
 };
 constexpr int MAX_GROUPS = 256;   // groups whose (row, last key) a CTA keeps
 
-// Merge an item's pieces (and, after a shared prefix, the prefix's splits):
-// thread = 8 features of a query row; pieces in order.
+// 8 features of a query row on their way through partials.
+struct Joined {
+    float mx = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+};
+
+// Merge an item's pieces (and, after a shared prefix, the prefix's splits) by a
+// whole CTA: a thread takes 8 features of a query row and every P-th piece, in
+// order; P such threads then add up through shared memory (10 floats a thread).
 template <typename T, int D>
 __device__ __forceinline__ void join_item(const PagedKV &kv, const PagedQuery &a, int QR, size_t item,
-                                          const float *o_part, const float *ml_part, int2 mt, const PrefixPartials &pre) {
+                                          const float *o_part, const float *ml_part, int2 mt, const PrefixPartials &pre,
+                                          float *sm) {
     const int Hq = a.n_heads, G = Hq / kv.n_kv;
     const int qts = (a.qg * G + QR - 1) / QR, per_group = kv.n_kv * qts;
     const int grp = (int)(item / per_group), x = (int)(item % per_group), h = x / qts, qt = x - h * qts;
     if (mt.y < 0 && pre.splits == 0) return;   // written already
     const int t0 = grp * a.qg, ntok = min(a.qg, a.M - t0);
-    const int nq = min(QR, ntok * G - qt * QR);
+    const int nq = min(QR, ntok * G - qt * QR), W = nq * (D / 8);
     const int n_own = mt.y >= 0 ? mt.y - mt.x + 1 : 0, n = n_own + pre.splits;
+    if (W <= 0) return;
     constexpr int PB = 8;   // pieces whose loads are in flight together
-    for (int w = threadIdx.x; w < nq * (D / 8); w += blockDim.x) {
-        const int r = w / (D / 8), d = (w % (D / 8)) * 8;
-        const int rr = qt * QR + r, m = t0 + rr / G;
-        if (__ldg(a.trow + m) < 0) continue;
-        float acc[8], l = 0.f, mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-        for (int p0 = 0; p0 < n; p0 += PB) {
+    auto gather = [&](int w, int first, int step, Joined &j) {
+        const int r = w / (D / 8), d = (w % (D / 8)) * 8, rr = qt * QR + r;
+        for (int p0 = first; p0 < n; p0 += PB * step) {
             float2 ml[PB];
             float4 va[PB], vb[PB];
 #pragma unroll
             for (int k = 0; k < PB; ++k) {
                 ml[k] = make_float2(-INFINITY, 0.f);
                 va[k] = vb[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                const int p = p0 + k;
+                const int p = p0 + k * step;
                 if (p < n) {
-                    size_t at;
-                    const float *os, *ms;
-                    if (p < n_own) {
-                        at = (item + mt.x + p) * QR + r;
-                        os = o_part; ms = ml_part;
-                    } else {
-                        at = ((size_t)(p - n_own) * kv.n_kv + h) * ((size_t)a.M * G) + (size_t)t0 * G + rr;
-                        os = pre.o; ms = pre.ml;
-                    }
+                    const bool own = p < n_own;
+                    const size_t at = own ? (item + mt.x + p) * QR + r
+                                          : ((size_t)(p - n_own) * kv.n_kv + h) * ((size_t)a.M * G) + (size_t)t0 * G + rr;
+                    const float *os = own ? o_part : pre.o, *ms = own ? ml_part : pre.ml;
                     ml[k] = *reinterpret_cast<const float2 *>(ms + at * 2);
                     va[k] = *reinterpret_cast<const float4 *>(os + at * D + d);
                     vb[k] = *reinterpret_cast<const float4 *>(os + at * D + d + 4);
                 }
             }
-            float mb = mx;
+            float mb = j.mx;
 #pragma unroll
             for (int k = 0; k < PB; ++k) mb = fmaxf(mb, ml[k].x);
-            if (mx != -INFINITY && mx != mb) {
-                const float f = tc::ex2_approx(mx - mb);
-                l *= f;
+            if (j.mx != -INFINITY && j.mx != mb) {
+                const float f = tc::ex2_approx(j.mx - mb);
+                j.l *= f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] *= f;
+                for (int i = 0; i < 8; ++i) j.acc[i] *= f;
             }
-            mx = mb;
+            j.mx = mb;
 #pragma unroll
             for (int k = 0; k < PB; ++k) {
                 const float f = weight_of(ml[k].x, ml[k].y, mb);
-                l += f * ml[k].y;
-                acc[0] += f * va[k].x; acc[1] += f * va[k].y; acc[2] += f * va[k].z; acc[3] += f * va[k].w;
-                acc[4] += f * vb[k].x; acc[5] += f * vb[k].y; acc[6] += f * vb[k].z; acc[7] += f * vb[k].w;
+                j.l += f * ml[k].y;
+                j.acc[0] += f * va[k].x; j.acc[1] += f * va[k].y; j.acc[2] += f * va[k].z; j.acc[3] += f * va[k].w;
+                j.acc[4] += f * vb[k].x; j.acc[5] += f * vb[k].y; j.acc[6] += f * vb[k].z; j.acc[7] += f * vb[k].w;
             }
         }
-        const float inv = l != 0.f ? 1.f / l : 0.f;
+    };
+    auto write = [&](int w, const Joined &j) {
+        const int r = w / (D / 8), d = (w % (D / 8)) * 8, rr = qt * QR + r, m = t0 + rr / G;
+        if (__ldg(a.trow + m) < 0) return;
+        const float inv = j.l != 0.f ? 1.f / j.l : 0.f;
         uint4 y;
-        y.x = Half2<T>::pack(acc[0] * inv, acc[1] * inv);
-        y.y = Half2<T>::pack(acc[2] * inv, acc[3] * inv);
-        y.z = Half2<T>::pack(acc[4] * inv, acc[5] * inv);
-        y.w = Half2<T>::pack(acc[6] * inv, acc[7] * inv);
+        y.x = Half2<T>::pack(j.acc[0] * inv, j.acc[1] * inv);
+        y.y = Half2<T>::pack(j.acc[2] * inv, j.acc[3] * inv);
+        y.z = Half2<T>::pack(j.acc[4] * inv, j.acc[5] * inv);
+        y.w = Half2<T>::pack(j.acc[6] * inv, j.acc[7] * inv);
         *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr % G) * D + d) = y;
+    };
+    const int P = min((int)blockDim.x / W, n);
+    if (P <= 1) {
+        for (int w = threadIdx.x; w < W; w += blockDim.x) {
+            Joined j;
+            gather(w, 0, 1, j);
+            write(w, j);
+        }
+        return;
     }
+    const int g = threadIdx.x / W, w = threadIdx.x % W;
+    Joined j;
+    if (g < P) gather(w, g, P, j);
+    float *mine = sm + threadIdx.x;
+    const int bs = blockDim.x;
+    mine[0] = j.mx;
+    mine[bs] = j.l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mine[(2 + i) * bs] = j.acc[i];
+    __syncthreads();
+    if (g == 0) {
+        float mx = j.mx;
+        for (int p = 1; p < P; ++p) mx = fmaxf(mx, sm[p * W + w]);
+        Joined t;
+        for (int p = 0; p < P; ++p) {
+            const float *o = sm + p * W + w;
+            const float f = weight_of(o[0], o[bs], mx);
+            t.l += f * o[bs];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t.acc[i] += f * o[(2 + i) * bs];
+        }
+        write(w, t);
+    }
+    __syncthreads();   // before the next item's
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 attn_join(const PagedKV kv, const PagedQuery a, int QR, const float *__restrict__ o_part,
           const float *__restrict__ ml_part, const int2 *__restrict__ meta, const PrefixPartials pre) {
+    __shared__ float sm[10 * 256];
     griddep_launch_dependents();
     griddep_wait();
-    join_item<T, D>(kv, a, QR, blockIdx.x, o_part, ml_part, meta[blockIdx.x], pre);
+    join_item<T, D>(kv, a, QR, blockIdx.x, o_part, ml_part, meta[blockIdx.x], pre, sm);
 }
 
 template <typename T, int D, int NT>
@@ -638,7 +674,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         // a call of few units is one cluster: it joins its pieces itself, behind a
         // barrier that also orders their stores
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-        for (size_t i = blockIdx.x; i < (size_t)items; i += gridDim.x) join_item<T, D>(kv, a, S::QR, i, o_part, ml_part, meta[i], pre);
+        for (size_t i = blockIdx.x; i < (size_t)items; i += gridDim.x) join_item<T, D>(kv, a, S::QR, i, o_part, ml_part, meta[i], pre, reinterpret_cast<float *>(psm));
     }
 }
 
@@ -711,8 +747,7 @@ cudaError_t run(const PagedKV &kv, const PagedQuery &q, int key_begin, const Pre
         default: e = launch_main<T, D, 4>(kv, q, key_begin, pre, s, ws, grid, cluster, st); break;
     }
     if (e != cudaSuccess || cluster) return e;
-    const int threads = std::min(256, (NT * 8 * (D / 8) + 31) / 32 * 32);
-    return launch_pdl(attn_join<T, D>, dim3((unsigned)s.items), dim3(threads), 0, st, kv, q, NT * 8,
+    return launch_pdl(attn_join<T, D>, dim3((unsigned)s.items), dim3(256), 0, st, kv, q, NT * 8,
                       (const float *)ws, (const float *)(ws + s.ml_at), (const int2 *)(ws + s.meta_at), pre);
 }
 
