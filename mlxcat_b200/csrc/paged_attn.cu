@@ -53,6 +53,7 @@ struct Half2<__half> {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t *>(&h);
     }
+    static __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
     static constexpr uint32_t ones = 0x3C003C00u;
     static __device__ __forceinline__ void mma(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -66,6 +67,7 @@ struct Half2<__nv_bfloat16> {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t *>(&h);
     }
+    static __device__ __forceinline__ float2 unpack(uint32_t x) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&x)); }
     static constexpr uint32_t ones = 0x3F803F80u;
     static __device__ __forceinline__ void mma(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -268,6 +270,10 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
     using S = PagedShape<D, NT>;
     constexpr int CH = D / 8;            // 16-byte chunks per key
     constexpr int RPI = 32 / CH;         // keys per load instruction of a warp
+    // Up to three n8 tiles the kernel waits for HBM, not for the tensor cores: P goes in
+    // as two 16-bit parts and keeps 21 (bf16: 16) bits, so the result's own rounding is
+    // the only one that shows.
+    constexpr bool TWO = NT <= 3;
     extern __shared__ __align__(128) unsigned char psm[];
     unsigned char *qsm = psm + S::BODY;                                       // [QR][D], chunks swizzled
     int *lim_s = reinterpret_cast<int *>(qsm + S::QR * D * 2);                // [QR]
@@ -554,16 +560,27 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
                         }
                     }
             }
-            uint32_t pb[NT][2];
+            uint32_t pb[NT][2], pl[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float n0 = mr[nt][0] == -INFINITY ? 0.f : mr[nt][0], n1 = mr[nt][1] == -INFINITY ? 0.f : mr[nt][1];
-                pb[nt][0] = turn8x8(Half2<T>::pack(tc::ex2_approx(sc[nt][0] - n0), tc::ex2_approx(sc[nt][1] - n1)));
-                pb[nt][1] = turn8x8(Half2<T>::pack(tc::ex2_approx(sc[nt][2] - n0), tc::ex2_approx(sc[nt][3] - n1)));
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float p0 = tc::ex2_approx(sc[nt][2 * e] - n0), p1 = tc::ex2_approx(sc[nt][2 * e + 1] - n1);
+                    const uint32_t hi = Half2<T>::pack(p0, p1);
+                    pb[nt][e] = turn8x8(hi);
+                    if (TWO) {   // what the rounding left out
+                        const float2 h = Half2<T>::unpack(hi);
+                        pl[nt][e] = turn8x8(Half2<T>::pack(p0 - h.x, p1 - h.y));
+                    }
+                }
             }
             const uint32_t one[4] = {Half2<T>::ones, Half2<T>::ones, Half2<T>::ones, Half2<T>::ones};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) Half2<T>::mma(ls[nt], one, pb[nt][0], pb[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+                Half2<T>::mma(ls[nt], one, pb[nt][0], pb[nt][1]);
+                if (TWO) Half2<T>::mma(ls[nt], one, pl[nt][0], pl[nt][1]);
+            }
             {
                 const int r = (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
@@ -571,7 +588,10 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
                     uint32_t f[4];
                     ldm4t(f, va + (uint32_t)(r * D * 2 + (((mt * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4)));
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) Half2<T>::mma(o[mt][nt], f, pb[nt][0], pb[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        Half2<T>::mma(o[mt][nt], f, pb[nt][0], pb[nt][1]);
+                        if (TWO) Half2<T>::mma(o[mt][nt], f, pl[nt][0], pl[nt][1]);
+                    }
                 }
             }
         }

@@ -374,12 +374,14 @@ def test_paged_attention_scale_and_large_scores():
         cache.put(r, k * torch.linspace(0.1, 6.0, n, device="cuda").to(k.dtype)[:, None, None], v)
     trow, tpos = ints([0, 1]), ints([699, 89])
     q = rnd((2, 8, 64), g, "bf16", 3.0)
-    for prefix in (None, 64):
+    for prefix, copies in ((None, 1), (64, 1), (64, 5000)):   # per row, and once for all
         if prefix:
             table[1, :2] = table[0, :2]
-        out = torch.full_like(q, 9.0)
-        A.check(paged(cache, q, 1, trow, tpos, out, prefix, scale=0.3))
-        check_rows(cache, q, 1, trow, tpos, out, "bf16", 0.3)
+        qq, rr, pp = q.repeat(copies, 1, 1), trow.repeat(copies), tpos.repeat(copies)
+        out = torch.full_like(qq, 9.0)
+        A.check(paged(cache, qq, 1, rr, pp, out, prefix, scale=0.3))
+        check_rows(cache, q, 1, trow, tpos, out[-2:], "bf16", 0.3)
+        check_rows(cache, q, 1, trow, tpos, out[copies // 2 * 2:][:2], "bf16", 0.3)
 
 
 def test_paged_attention_far_pages():
@@ -398,18 +400,15 @@ def test_paged_attention_far_pages():
                    ints(list(range(700))), q_out))
     kk, vv = cache.row(0, 700)
     assert torch.equal(kk.reshape(700, -1), x[:, 2 * hk * d:3 * hk * d].half()) and torch.equal(vv.reshape(700, -1), x[:, 3 * hk * d:].half())
-    for prefix in (None, 512):
-        out = torch.full((1, 4, d), 9.0, dtype=torch.float16, device="cuda")
-        A.check(paged(cache, q_out[:1].contiguous(), 1, ints([0]), ints([699]), out, prefix))
-        check_rows(cache, q_out[:1], 1, ints([0]), ints([699]), out, "f16")
+    for prefix, copies in ((None, 1), (512, 1), (512, 300)):   # per row, and once for all
+        q = q_out[:1].repeat(copies, 1, 1)
+        out = torch.full_like(q, 9.0)
+        A.check(paged(cache, q, 1, ints([0] * copies), ints([699] * copies), out, prefix))
+        check_rows(cache, q[:1], 1, ints([0]), ints([699]), out[-1:], "f16")
 
 
 # ------------------------------------------------------------------------------------------ shared prefix
-@pytest.mark.parametrize("h,hk,d,dt,qg,ps,prefix,rows,nhd", [
-    (8, 2, 64, "f16", 1, 16, 48, 3, False), (32, 8, 128, "bf16", 1, 256, 2048, 40, False), (32, 8, 128, "f16", 5, 64, 320, 9, True),
-    (32, 4, 128, "bf16", 4, 8, 2056, 20, False), (10, 2, 64, "bf16", 2, 32, 416, 30, True), (64, 1, 128, "f16", 1, 128, 1024, 5, False),
-    (4, 4, 128, "f16", 1, 16, 16, 1, False), (48, 16, 64, "f16", 3, 8, 136, 70, False)])
-def test_shared_prefix_attention(h, hk, d, dt, qg, ps, prefix, rows, nhd):
+def shared_case(h, hk, d, dt, qg, ps, prefix, rows, nhd, sample=None):
     g = gen(h + d + rows)
     own = [(1, 2, 63, 64, 65, 200)[r % 6] + qg - 1 for r in range(rows)]
     lens = [prefix + n for n in own]
@@ -428,10 +427,64 @@ def test_shared_prefix_attention(h, hk, d, dt, qg, ps, prefix, rows, nhd):
     A.check(paged(cache, q, qg, trow, tpos, out, prefix, err=err))
     torch.cuda.synchronize()
     assert err.item() == 0
-    check_rows(cache, q, qg, trow, tpos, out, dt)
+    m = len(trow)
+    at = torch.arange(m, device="cuda") if sample is None else torch.tensor(sorted({0, qg, m - 1, m - qg - 1} | {i * m // sample for i in range(sample)}),
+                                                                          device="cuda")
+    check_rows(cache, q[at], qg, trow[at], tpos[at], out[at], dt)
     again = torch.full_like(q, 9.0)
     A.check(paged(cache, q, qg, trow, tpos, again, prefix))
     assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("h,hk,d,dt,qg,ps,prefix,rows,nhd", [
+    (8, 2, 64, "f16", 1, 16, 48, 3, False), (32, 8, 128, "f16", 5, 64, 320, 9, True), (64, 1, 128, "f16", 1, 128, 1024, 5, False),
+    (4, 4, 128, "f16", 1, 16, 16, 1, False), (48, 16, 64, "f16", 3, 8, 136, 70, False)])
+def test_shared_prefix_attention_read_per_row(h, hk, d, dt, qg, ps, prefix, rows, nhd):
+    assert rows * prefix * hk * d * 4 <= 128 << 20
+    shared_case(h, hk, d, dt, qg, ps, prefix, rows, nhd)
+
+
+@pytest.mark.parametrize("h,hk,d,dt,qg,ps,prefix,rows,nhd", [
+    (32, 8, 128, "bf16", 1, 256, 2048, 40, False),      # page of two blocks, whole blocks
+    (32, 4, 128, "bf16", 4, 8, 2056, 40, False),        # last block of 8 keys, pages of 8
+    (10, 2, 64, "bf16", 2, 32, 4000, 70, True),         # last block of 32 keys, token-major pages
+    (64, 1, 128, "f16", 1, 128, 2944, 97, False),       # 2 tokens fill a tile
+    (4, 4, 128, "f16", 1, 16, 1040, 70, True),          # one head a group, last block of 16 keys
+    (48, 16, 64, "f16", 3, 8, 1000, 37, False),
+    (33, 1, 64, "f16", 1, 64, 16384, 33, False),        # rows of a tile that no token owns
+    (8, 8, 64, "bf16", 8, 1024, 5120, 20, False)])
+def test_shared_prefix_attention_read_once(h, hk, d, dt, qg, ps, prefix, rows, nhd):
+    assert rows * prefix * hk * d * 4 > 128 << 20
+    shared_case(h, hk, d, dt, qg, ps, prefix, rows, nhd, sample=24)
+
+
+def test_shared_prefix_attention_bad_page():
+    """A page of the prefix outside the cache sets the flag and reads as zeros."""
+    rows, hk, d, ps, prefix = 70, 4, 128, 256, 1024
+    lens = [prefix + 5] * rows
+    table, n_pages = tables(lens, ps, lead=(0,) * (prefix // ps))
+    cache = Paged(hk, d, ps, n_pages, "bf16", table)
+    g = gen(1)
+    fill_rows(cache, lens, g, "bf16", shared=prefix)
+    q = rnd((rows, 8, d), g, "bf16")
+    trow, tpos = ints(list(range(rows))), ints([n - 1 for n in lens])
+    for bad in (-1, n_pages, 2 ** 31 - 1):
+        table[:, 1] = bad
+        out, err = torch.full_like(q, 9.0), ints([0])
+        A.check(paged(cache, q, 1, trow, tpos, out, prefix, err=err))
+        torch.cuda.synchronize()
+        assert err.item() != 0
+        k, v = (torch.cat([x[:256], torch.zeros_like(x[:256]), x[512:]]) for x in (lambda t: (t[0], t[1]))(cache_row_with(cache, 3, lens[3], 1)))
+        check(out[3:4], attend64(q[3:4], k, v, tpos[3:4].long()), "bf16", q[3:4], k, v)
+
+
+def cache_row_with(cache, row, n, hole):
+    """A row's keys and values with page `hole` of its table read as page 0 (the caller blanks it)."""
+    keep = cache.table[row, hole].item()
+    cache.table[row, hole] = 0
+    k, v = cache.row(row, n)
+    cache.table[row, hole] = keep
+    return k, v
 
 
 # ------------------------------------------------------------------------------------------------- packed
@@ -508,6 +561,28 @@ def test_packed_attention_large_scores_and_scale():
     check_packed(q, k, v, cu, cu, 1, out, "bf16", 0.3)
 
 
+@pytest.mark.parametrize("n,h,hk,d,dt", [(31, 8, 2, 64, "f16"), (100, 32, 8, 128, "bf16"), (1500, 4, 2, 64, "f16"), (33, 16, 1, 128, "f16")])
+def test_packed_attention_many_sequences(n, h, hk, d, dt):
+    """More items than SMs, more sequences than one round of the search; empty ones among them."""
+    g = torch.Generator().manual_seed(n)
+    top = 300 if n <= 100 else 9
+    lens = torch.randint(0, top, (n,), generator=g)
+    past = torch.randint(0, 200, (n,), generator=g) * (torch.rand(n, generator=g) < 0.5)
+    lens[n // 2] = 0
+    cu_q, cu_k = ints([0] + lens.cumsum(0).tolist()), ints([0] + (lens + past).cumsum(0).tolist())
+    gc = gen(n)
+    tq, tk = int(lens.sum()), int((lens + past).sum())
+    q, k, v = rnd((tq, h, d), gc, dt), rnd((tk, hk, d), gc, dt), rnd((tk, hk, d), gc, dt)
+    out, err = torch.full_like(q, 9.0), ints([0])
+    A.check(packed(q, k, v, cu_q, cu_k, 1, out, dt, err=err))
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    check_packed(q, k, v, cu_q, cu_k, 1, out, dt)
+    again = torch.full_like(q, 9.0)
+    A.check(packed(q, k, v, cu_q, cu_k, 1, again, dt))
+    assert torch.equal(out, again)
+
+
 def test_packed_attention_bad_offsets_stay_inside():
     """Offsets past the buffers are cut to them: finite results, nothing written outside the queries."""
     g = gen(7)
@@ -565,6 +640,42 @@ def test_graph_replay_and_two_streams():
     torch.cuda.synchronize()
     for qq, o in zip(qs, outs):
         check_rows(cache, qq, 1, trow, tpos, o, dt)
+
+
+def test_graph_of_packed_and_shared_attention():
+    """Both tensor-core paths captured together and replayed on new values and lengths."""
+    g, dt, h, hk, d, ps, rows, prefix = gen(11), "bf16", 16, 4, 128, 64, 40, 2048
+    lens = [prefix + 3 + r for r in range(rows)]
+    table, n_pages = tables([n + 4 for n in lens], ps, lead=(0,) * (prefix // ps))
+    cache = Paged(hk, d, ps, n_pages, dt, table)
+    fill_rows(cache, [n + 4 for n in lens], g, dt, shared=prefix)
+    trow, tpos = ints(list(range(rows))), ints([n - 1 for n in lens])
+    q, out = rnd((rows, h, d), g, dt), torch.zeros((rows, h, d), dtype=DT[dt], device="cuda")
+    ws = torch.empty(L.mlxcat_op_shared_prefix_attention_workspace(rows, 1, h, hk, d, prefix), dtype=torch.uint8, device="cuda")
+    pq, pk, pv = rnd((700, h, d), g, dt), rnd((700, hk, d), g, dt), rnd((700, hk, d), g, dt)
+    cu, po = ints([0, 100, 101, 700]), torch.zeros((700, h, d), dtype=DT[dt], device="cuda")
+
+    def step():
+        A.check(packed(pq, pk, pv, cu, cu, 1, po, dt))
+        A.check(paged(cache, q, 1, trow, tpos, out, prefix, ws=ws))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(3):
+        q.copy_(rnd(q.shape, g, dt))
+        pq.copy_(rnd(pq.shape, g, dt))
+        cu.copy_(ints([[0, 100, 101, 700], [0, 0, 333, 700], [0, 650, 651, 700]][i]))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_rows(cache, q[::7], 1, trow[::7], tpos[::7], out[::7], dt)
+        check_packed(pq, pk, pv, cu, cu, 1, po, dt)
+        tpos += 1
 
 
 # -------------------------------------------------------------------------------------- a serving run
