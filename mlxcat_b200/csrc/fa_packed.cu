@@ -141,6 +141,11 @@ __device__ __forceinline__ void store32(void *p, const uint32_t *v) {
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
+__device__ __forceinline__ void prefetch_3d(const CUtensorMap *map, int x, int y, int z) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];\n" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+                 "r"(y), "r"(z) : "memory");
+}
+
 template <typename T>
 struct Pk;
 template <>
@@ -356,18 +361,26 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 ++it;
             }
             if (w.ntok > 0 && w.nb) {
-                for (int i = 0; i < w.tiles && ok; ++i) {
-                    int &qc = i ? qc1 : qc0;
-                    if (qc) ok = wait_all(fb.q_free[i], qc - 1, abort, a.err, PK_FREE);
-                    if (ok && lane == 0) {
-                        const uint32_t qb = tc::smem_u32(&fb.q_full[i]);
-                        tc::mbar_arrive_expect_tx(qb, (uint32_t)(S::HALVES * a.G * a.TQ * 128));
-                        for (int x = 0; x < S::HALVES; ++x)
-                            tc::tma_load_3d(tc::smem_u32(sm_q + i * S::TILE + x * BOX), &qmap, x * 64, w.h * a.G, w.tok0 + i * a.TQ, qb);
+                // the queries' memory is free only when the last item's scores are through:
+                // bring them to L2 meanwhile, and the first K, which has room earlier, in
+                if (lane < w.tiles * S::HALVES)
+                    prefetch_3d(&qmap, (lane % S::HALVES) * 64, w.h * a.G, w.tok0 + lane / S::HALVES * a.TQ);
+                auto load_q = [&]() {
+                    for (int i = 0; i < w.tiles && ok; ++i) {
+                        int &qc = i ? qc1 : qc0;
+                        if (qc) ok = wait_all(fb.q_free[i], qc - 1, abort, a.err, PK_FREE);
+                        if (ok && lane == 0) {
+                            const uint32_t qb = tc::smem_u32(&fb.q_full[i]);
+                            tc::mbar_arrive_expect_tx(qb, (uint32_t)(S::HALVES * a.G * a.TQ * 128));
+                            for (int x = 0; x < S::HALVES; ++x)
+                                tc::tma_load_3d(tc::smem_u32(sm_q + i * S::TILE + x * BOX), &qmap, x * 64, w.h * a.G, w.tok0 + i * a.TQ, qb);
+                        }
+                        if (ok) ++qc;
                     }
-                    if (ok) ++qc;
-                }
-                for (int f = 0; f < 2 * w.nb && ok; ++f) {   // K_0, V_0, K_1, ...
+                };
+                for (int f = 0; f < 2 * w.nb && ok; ++f) {   // K_0, the queries, V_0, K_1, ...
+                    if (f == 1) load_q();
+                    if (!ok) break;
                     const int j = f >> 1, v = f & 1, fill = v ? vc : kc, s = v ? fill % VSLOTS : fill % KSLOTS, turn = v ? fill / VSLOTS : fill / KSLOTS;
                     if (turn) ok = wait_all(v ? fb.v_free[s] : fb.k_free[s], turn - 1, abort, a.err, PK_FREE);
                     if (!ok) break;
