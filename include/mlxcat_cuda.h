@@ -478,7 +478,9 @@ MLXCAT_API int mlxcat_op_paged_attention(const mlxcat_paged_kv *kv, const void *
 /* The same result for a batch whose rows share their first prefix_len keys
  * (a multiple of page_size; page_table[r] starts with the same prefix_len /
  * page_size pages for every row r of the batch): those pages are read once for
- * all tokens, on the tensor cores.  prefix_len 0 is mlxcat_op_paged_attention. */
+ * all tokens, on the tensor cores.  prefix_len 0 is mlxcat_op_paged_attention,
+ * and so is a call whose rows would together read at most 128 MB of the prefix
+ * (L2 serves that faster than a second pass and a join). */
 MLXCAT_API size_t mlxcat_op_shared_prefix_attention_workspace(int32_t M, int32_t qg, int32_t n_heads,
                                                               int32_t n_kv_heads, int32_t head_dim,
                                                               int32_t prefix_len);

@@ -22,6 +22,13 @@
 //   takes an equal stretch.  An item inside one CTA is finished there; the
 //   others leave (O, max, sum) partials, which attn_join merges in order, so
 //   results do not depend on timing.
+//
+// Two CTAs of four warps an SM keep 128 KB of loads in flight; with two or one
+// warp a CTA (four or six CTAs) 64 rows of up to 16k keys took 395 and 308 us
+// against 298.  Measured on one B200: those 64 rows (64 query heads, 8 KV heads of
+// 128, bf16) 298 us, 6.3 TB/s, 0.97 of the copy rate; 32 x 5 verify tokens over
+// 4.2k keys 103 us, 5.3 TB/s.  What is left there is the start (the lengths, the
+// page ids and the first keys are one chain of loads, 3 us) and the join.
 #include <algorithm>
 
 #include "common.cuh"
@@ -270,10 +277,11 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
     using S = PagedShape<D, NT>;
     constexpr int CH = D / 8;            // 16-byte chunks per key
     constexpr int RPI = 32 / CH;         // keys per load instruction of a warp
-    // Up to three n8 tiles the kernel waits for HBM, not for the tensor cores: P goes in
+    // Up to two n8 tiles the kernel waits for HBM, not for the tensor cores: P goes in
     // as two 16-bit parts and keeps 21 (bf16: 16) bits, so the result's own rounding is
-    // the only one that shows.
-    constexpr bool TWO = NT <= 3;
+    // the only one that shows (64 single tokens over up to 16k keys: 298 us either way).
+    // With three tiles it cost 105 -> 117 us at 32 x 5 tokens over 4.2k keys.
+    constexpr bool TWO = NT <= 2;
     extern __shared__ __align__(128) unsigned char psm[];
     unsigned char *qsm = psm + S::BODY;                                       // [QR][D], chunks swizzled
     int *lim_s = reinterpret_cast<int *>(qsm + S::QR * D * 2);                // [QR]

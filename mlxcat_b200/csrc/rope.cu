@@ -10,10 +10,17 @@
 // turns (pos * f_i / 2 pi, the integer part dropped), so a position of 2^31
 // still has its fraction to 2^-22 of a turn; only the fraction goes to fp32.
 //
-// Bound by HBM: every input is read and every output written once.  One CTA per
-// token: its r/2 angles are computed once for all its heads.  A thread owns 8
-// consecutive features (16-byte stores); a head is D/8 neighbouring lanes, so
-// the sum of squares and the rotation partner of the half layout are shuffles.
+// Every input is read and every output written once.  A warp takes one token, or
+// some of its heads when tokens are few, forms the angles once (a lane two pairs,
+// through shared memory) and goes over the heads with the next ones' loads in
+// flight.  A lane owns features d0..d0+7 and D/2 + d0..+7 of a head: the half
+// layout's partners over the whole head are then in one lane, the sum of squares
+// needs three shuffles (D = 128), and every access is 16 bytes.  A CTA per token
+// spent most of its time on the chain position -> angles -> barrier (133 us for
+// 16,396 tokens of 32 + 2 * 8 heads, bf16, normalised, interleaved), groups of four
+// tokens a CTA still on the barrier (89 us); now 80 us, 5.0 TB/s, 0.77 of the copy
+// rate, and what bounds it is the instruction rate (65 % of issue slots; without
+// the norms 68 us).  160 tokens of an fp32 projection: 4.5 us, launch-bound.
 #include <algorithm>
 
 #include "common.cuh"
