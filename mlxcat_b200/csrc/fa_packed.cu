@@ -63,6 +63,7 @@ constexpr int KB = 128;                 // keys of a block
 constexpr int BOX = 128 * 128;          // [128 rows][64 features] swizzled
 constexpr int KSLOTS = 2, VSLOTS = 3;   // rings of K and V blocks
 constexpr int THREADS = 416;
+constexpr int FEW_BLOCKS = 8;           // key blocks a CTA of a prefix pass below which it takes half the SMs
 constexpr int SB = 64;                  // keys of a score buffer: two per tile
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
@@ -652,7 +653,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             if (!ok) break;
             const float inv = l != 0.f ? 1.f / l : 0.f;
             T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(w.tok0 + tk) * a.Hq + w.h * a.G + gh) * D;
-            const size_t prow = ((size_t)w.split * a.Hkv + w.h) * ((size_t)a.M * a.G) + (size_t)(w.tok0 + tk) * a.G + gh;
+            const size_t part_rows = (size_t)a.M * a.G, part_row = (size_t)(w.tok0 + tk) * a.G + gh;
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.work_free[it & 1]));
 #pragma unroll 1
@@ -673,9 +674,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 for (int x = 0; x < 32; ++x)
                     if (!live) acc[x] = 0u;
                 if (!pad && a.prefix) {
-                    float *p = a.o_part + prow * D + c * 32;
+                    // [split][KV head][8 features][row][8]: a warp's 32 rows are one kilobyte
+                    float *p = a.o_part + (((size_t)w.split * a.Hkv + w.h) * (D / 8) + c * 4) * part_rows * 8 + part_row * 8;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) store32(p + x * 8, acc + x * 8);
+                    for (int x = 0; x < 4; ++x) store32(p + x * part_rows * 8, acc + x * 8);
                 } else if (!pad) {
                     uint32_t y[16];
 #pragma unroll
@@ -691,7 +693,8 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     }
                 }
             }
-            if (a.prefix && !pad) *reinterpret_cast<float2 *>(a.ml_part + prow * 2) = make_float2(m_used, l);
+            if (a.prefix && !pad)
+                *reinterpret_cast<float2 *>(a.ml_part + (((size_t)w.split * a.Hkv + w.h) * part_rows + part_row) * 2) = make_float2(m_used, l);
         }
     }
     tc::fence_before_sync();
@@ -768,11 +771,24 @@ cudaError_t packed_attn(const PackedAttn &p, cudaStream_t st) {
     return launch_any(qm, km, vm, a, p.D, p.bf16, tiles * p.n_kv, st);
 }
 
+int prefix_items(int M, int n_heads, int n_kv) {
+    const int TQ = TM / (n_heads / n_kv);
+    return (int)std::min<int64_t>((int64_t)((M + 2 * TQ - 1) / (2 * TQ)) * n_kv, 0x7fffffff);
+}
+
 int prefix_splits(int M, int n_heads, int n_kv, int prefix_len, int sm_count) {
-    const int G = n_heads / n_kv, TQ = TM / G;
-    const int64_t items = (int64_t)((M + 2 * TQ - 1) / (2 * TQ)) * n_kv;
-    const int blocks = (prefix_len + KB - 1) / KB;
-    // one wave of CTAs, two key blocks each at least
+    const int64_t items = prefix_items(M, n_heads, n_kv), blocks = (prefix_len + KB - 1) / KB;
+    // one wave of CTAs, two key blocks each at least; half a wave when a whole one
+    // would have few blocks each: start and end of a CTA then count for more than
+    // its blocks, and the rows' own keys are read on the other SMs meanwhile (64
+    // tokens over 8,192 shared keys: 46.7 us on all, 44.5 on a third, 41.3 on half)
+    int64_t sms = sm_count;
+    if (blocks * items < FEW_BLOCKS * sms) sms /= 2;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(sms / items, (blocks + 1) / 2));
+}
+
+int prefix_max_splits(int M, int n_heads, int n_kv, int prefix_len, int sm_count) {
+    const int64_t items = prefix_items(M, n_heads, n_kv), blocks = (prefix_len + KB - 1) / KB;
     return (int)std::max<int64_t>(1, std::min<int64_t>(sm_count / items, (blocks + 1) / 2));
 }
 

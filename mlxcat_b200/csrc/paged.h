@@ -57,11 +57,11 @@ struct PagedQuery {
     int32_t *err;
 };
 
-// Partials of a shared-prefix pass: [splits][n_kv][M * G] rows of D fp32 sums
-// and (max, sum) pairs.
+// Partials of a shared-prefix pass: fp32 sums [splits][n_kv][D / 8][M * G rows][8]
+// and (max, sum) pairs [splits][n_kv][M * G].
 struct PrefixPartials {
     float *o = nullptr, *ml = nullptr;
-    int splits = 0;
+    int splits = 0, ctas = 0;   // CTAs of the pass
 };
 
 size_t paged_attn_scratch(int M, int qg, int n_heads, int n_kv, int D, int sm_count);
@@ -81,7 +81,9 @@ struct PackedAttn {
 };
 cudaError_t packed_attn(const PackedAttn &a, cudaStream_t st);
 
+int prefix_items(int M, int n_heads, int n_kv);   // CTAs of the pass per split
 int prefix_splits(int M, int n_heads, int n_kv, int prefix_len, int sm_count);
+int prefix_max_splits(int M, int n_heads, int n_kv, int prefix_len, int sm_count);   // at most, on so many SMs or fewer
 cudaError_t prefix_attn(const PagedKV &kv, const PagedQuery &q, int prefix_len, const PrefixPartials &part,
                         cudaStream_t st);
 

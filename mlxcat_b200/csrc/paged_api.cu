@@ -83,7 +83,8 @@ struct PrefixLayout {
 };
 PrefixLayout prefix_layout(int M, int n_heads, int n_kv, int D, int prefix_len) {
     PrefixLayout p;
-    p.splits = prefix_splits(M, n_heads, n_kv, prefix_len, SM_MAX);
+    // the workspace is sized before the device is known
+    p.splits = prefix_max_splits(M, n_heads, n_kv, prefix_len, SM_MAX);
     const size_t rows = (size_t)p.splits * M * n_heads;   // n_kv * (M * G)
     p.ml_at = up256(rows * D * 4);
     p.bytes = p.ml_at + up256(rows * 8);
@@ -254,6 +255,7 @@ int mlxcat_op_shared_prefix_attention(const mlxcat_paged_kv *c, int32_t prefix_l
         pre.o = reinterpret_cast<float *>(at);
         pre.ml = reinterpret_cast<float *>(at + l.ml_at);
         pre.splits = std::min(l.splits, prefix_splits(M, n_heads, kv.n_kv, prefix_len, std::min(sms, SM_MAX)));
+        pre.ctas = (int)std::min<int64_t>((int64_t)pre.splits * prefix_items(M, n_heads, kv.n_kv), 0x7fffffff);
         const cudaError_t e = prefix_attn(kv, pq, prefix_len, pre, st);
         if (e != cudaSuccess) return op_error(MLXCAT_E_CUDA, "shared prefix attention: %s", cudaGetErrorString(e));
     }

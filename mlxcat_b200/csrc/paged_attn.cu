@@ -186,13 +186,19 @@ __device__ __forceinline__ void join_item(const PagedKV &kv, const PagedQuery &a
                 va[k] = vb[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 const int p = p0 + k * step;
                 if (p < n) {
-                    const bool own = p < n_own;
-                    const size_t at = own ? (item + mt.x + p) * QR + r
-                                          : ((size_t)(p - n_own) * kv.n_kv + h) * ((size_t)a.M * G) + (size_t)t0 * G + rr;
-                    const float *os = own ? o_part : pre.o, *ms = own ? ml_part : pre.ml;
-                    ml[k] = *reinterpret_cast<const float2 *>(ms + at * 2);
-                    va[k] = *reinterpret_cast<const float4 *>(os + at * D + d);
-                    vb[k] = *reinterpret_cast<const float4 *>(os + at * D + d + 4);
+                    const float *o, *q;
+                    if (p < n_own) {
+                        const size_t at = (item + mt.x + p) * QR + r;
+                        o = o_part + at * D + d;
+                        q = ml_part + at * 2;
+                    } else {   // [split][KV head][8 features][row][8]
+                        const size_t rows = (size_t)a.M * G, sh = (size_t)(p - n_own) * kv.n_kv + h, row = (size_t)t0 * G + rr;
+                        o = pre.o + ((sh * (D / 8) + d / 8) * rows + row) * 8;
+                        q = pre.ml + (sh * rows + row) * 2;
+                    }
+                    ml[k] = *reinterpret_cast<const float2 *>(q);
+                    va[k] = *reinterpret_cast<const float4 *>(o);
+                    vb[k] = *reinterpret_cast<const float4 *>(o + 4);
                 }
             }
             float mb = j.mx;
@@ -764,9 +770,12 @@ cudaError_t run(const PagedKV &kv, const PagedQuery &q, int key_begin, const Pre
     // without a free SM would only start when the pass ends
     const int64_t cap = std::max(0, paged_capacity(kv) - key_begin);
     const int64_t units = (int64_t)s.items * ((cap + UNIT - 1) / UNIT + LEAD);
+    // Beside a prefix pass that leaves SMs free, this kernel takes those and no more:
+    // CTAs that had to wait for the pass would be the last.
+    const int free_sms = pre.splits && pre.ctas <= sm_count - sm_count / 4 ? sm_count - pre.ctas : sm_count;
     // few units: one cluster that joins its own pieces, no second kernel
     const bool cluster = units <= ONE_CLUSTER * CLUSTER_UNITS;
-    const int grid = (int)std::min<int64_t>(cluster ? ONE_CLUSTER : (int64_t)sm_count * CTAS_PER_SM, units);
+    const int grid = (int)std::min<int64_t>(cluster ? ONE_CLUSTER : (int64_t)free_sms * CTAS_PER_SM, units);
     cudaError_t e;
     switch (NT) {
         case 1: e = launch_main<T, D, 1>(kv, q, key_begin, pre, s, ws, grid, cluster, st); break;
