@@ -100,28 +100,32 @@ __device__ __forceinline__ void cpa16(uint32_t s, const void *g, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(g), "r"(bytes) : "memory");
 }
 
-// What a group of tokens sees: its row and one past its last key (clamped to
-// what the table holds).
+// What a group of tokens sees: its row and one past its last key.
 struct Group {
     int row, kend;
 };
+// the same, clamped to what the table holds; the flag where it was not
+__device__ __forceinline__ Group checked(const PagedKV &kv, const PagedQuery &a, Group x) {
+    const int cap = paged_capacity(kv);
+    if (x.row >= kv.rows || x.kend > cap) {
+        if (a.err) atomicExch(a.err, x.row >= kv.rows ? PE_ROW : PE_POS);
+        x.kend = x.row >= kv.rows ? 0 : cap;
+    }
+    if (x.row < 0) x.kend = 0;
+    return x;
+}
 __device__ __forceinline__ Group group_alone(const PagedKV &kv, const PagedQuery &a, int grp) {
     const int t0 = grp * a.qg, n = min(a.qg, a.M - t0);
-    int row = -1, kend = 0;
+    Group x = {-1, 0};
 #pragma unroll 4
     for (int j = 0; j < n; ++j) {
         const int r = __ldg(a.trow + t0 + j), p = __ldg(a.tpos + t0 + j);
         if (r >= 0) {
-            row = max(row, r);
-            kend = max(kend, p == 0x7fffffff ? p : p + 1);
+            x.row = max(x.row, r);
+            x.kend = max(x.kend, p == 0x7fffffff ? p : p + 1);
         }
     }
-    const int cap = paged_capacity(kv);
-    if (row >= kv.rows || kend > cap) {
-        if (a.err) atomicExch(a.err, row >= kv.rows ? PE_ROW : PE_POS);
-        kend = row >= kv.rows ? 0 : cap;
-    }
-    return {row, row < 0 ? 0 : kend};
+    return checked(kv, a, x);
 }
 
 __device__ __forceinline__ int64_t cta_begin(int c, int64_t U, int C) { return (int64_t)c * U / C; }
@@ -161,7 +165,7 @@ struct Joined {
 
 // Merge an item's pieces (and, after a shared prefix, the prefix's splits) by a
 // whole CTA: a thread takes 8 features of a query row and every P-th piece, in
-// order; P such threads then add up through shared memory (10 floats a thread).
+// order (P > 1 when there are more than one round of loads); P such threads then add up through shared memory (10 floats a thread).
 template <typename T, int D>
 __device__ __forceinline__ void join_item(const PagedKV &kv, const PagedQuery &a, int QR, size_t item,
                                           const float *o_part, const float *ml_part, int2 mt, const PrefixPartials &pre,
@@ -231,7 +235,7 @@ __device__ __forceinline__ void join_item(const PagedKV &kv, const PagedQuery &a
         y.w = Half2<T>::pack(j.acc[6] * inv, j.acc[7] * inv);
         *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr % G) * D + d) = y;
     };
-    const int P = min((int)blockDim.x / W, n);
+    const int P = min((int)blockDim.x / W, (n + PB - 1) / PB);
     if (P <= 1) {
         for (int w = threadIdx.x; w < W; w += blockDim.x) {
             Joined j;
@@ -316,11 +320,29 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
     const int per = (groups + PT - 1) / PT;
     const bool kept = groups <= MAX_GROUPS;
     int64_t mine = 0;
+    if (kept && a.qg > 1) {
+        // a thread per token, so that all loads are one round trip; a group's row and
+        // last key are maxima
+        for (int i = threadIdx.x; i < groups; i += PT) info[i] = {-1, 0};
+        __syncthreads();
+#pragma unroll 2
+        for (int m = threadIdx.x; m < a.M; m += PT) {
+            const int r = __ldg(a.trow + m), p = __ldg(a.tpos + m), i = m / a.qg;
+            if (r >= 0) {
+                atomicMax(&info[i].row, r);
+                atomicMax(&info[i].kend, p == 0x7fffffff ? p : p + 1);
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < groups; i += PT) info[i] = checked(kv, a, info[i]);
+        __syncthreads();
+    }
     {
         const int g0 = threadIdx.x * per, g1 = min(groups, g0 + per);
         for (int i = g0; i < g1; ++i) {
-            const Group x = group_alone(kv, a, i);
-            if (kept) info[i] = x;
+            const bool known = kept && a.qg > 1;
+            const Group x = known ? info[i] : group_alone(kv, a, i);
+            if (kept && !known) info[i] = x;
             mine += units_of(x);
         }
     }

@@ -18,9 +18,9 @@
 // needs three shuffles (D = 128), and every access is 16 bytes.  A CTA per token
 // spent most of its time on the chain position -> angles -> barrier (133 us for
 // 16,396 tokens of 32 + 2 * 8 heads, bf16, normalised, interleaved), groups of four
-// tokens a CTA still on the barrier (89 us); now 80 us, 5.0 TB/s, 0.77 of the copy
-// rate, and what bounds it is the instruction rate (65 % of issue slots; without
-// the norms 68 us).  160 tokens of an fp32 projection: 4.5 us, launch-bound.
+// tokens a CTA still on the barrier (89 us), a warp a token with every lane
+// choosing between q, k and v for itself 80 us; now 73 us, 5.5 TB/s, 0.84 of the
+// copy rate, and the instruction rate bounds it (70 % of issue slots).  160 tokens of an fp32 projection: 4.6 us, launch-bound.
 #include <algorithm>
 
 #include "common.cuh"
@@ -102,13 +102,15 @@ struct Vec8 {
 // half the head, half the rotary width a multiple of 8); ANY: read again.
 enum Partner { OWN, HALF, LANE, ANY };
 
-template <typename TI, typename TO, int D, int PARTNER>
+// MIXED: a round's heads may be of more than one kind (q, k, v); else the kind is
+// the round's and costs the lanes no selections.
+template <typename TI, typename TO, int D, int PARTNER, bool MIXED>
 __global__ void __launch_bounds__(RA_THREADS, ra_ctas<TI>())
 rope_append_kernel(const PagedKV kv, const __grid_constant__ mlxcat_rope rope, const RopeAppendArgs a, int chunks, int per) {
     constexpr int LPH = D / 16, HPI = 32 / LPH;   // lanes per head, heads of a warp at a time
     __shared__ __align__(16) float cosv[RA_THREADS / 32][D / 2], sinv[RA_THREADS / 32][D / 2];
     __shared__ __align__(16) float nw[2][D];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int nq = a.q ? a.n_heads : 0, heads = nq + 2 * kv.n_kv;
     const int j = lane % LPH, d0 = j * 8, hl0 = lane / LPH;
     const int half = a.with_rope ? rope.rotary_dim / 2 : 0;
@@ -131,9 +133,9 @@ rope_append_kernel(const PagedKV kv, const __grid_constant__ mlxcat_rope rope, c
         const int hb = h0 + round * HPI + hl0;
 #pragma unroll
         for (int b = 0; b < RA_BATCH; ++b) {
-            const int hh = hb + b * HPI;
-            if (round + b < per && hh < heads) {
-                const bool is_q = hh < nq, is_v = hh >= nq + kv.n_kv;
+            const int hh = hb + b * HPI, kd = MIXED ? hh : hh - hl0;
+            if (round + b < per && kd < heads) {
+                const bool is_q = kd < nq, is_v = kd >= nq + kv.n_kv;
                 const TI *p = reinterpret_cast<const TI *>(is_q ? a.q : is_v ? a.v : a.k) +
                               (int64_t)m * (int)(is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) +
                               (is_q ? hh : is_v ? hh - nq - kv.n_kv : hh - nq) * D + d0;
@@ -191,7 +193,8 @@ rope_append_kernel(const PagedKV kv, const __grid_constant__ mlxcat_rope rope, c
             for (int b = 0; b < RA_BATCH; ++b) {
                 const int hb = h0 + (round + b) * HPI, hh = hb + hl0;
                 if (!on || round + b >= per || hb >= heads) break;   // uniform: every lane shuffles
-                const bool in = hh < heads, is_q = hh < nq, is_v = hh >= nq + kv.n_kv;
+                const int kd = MIXED ? hh : hb;
+                const bool in = kd < heads, is_q = kd < nq, is_v = kd >= nq + kv.n_kv;
                 uint64_t x[2][4];
                 cur[b][0].get(x[0]);
                 cur[b][1].get(x[1]);
@@ -304,7 +307,9 @@ cudaError_t launch_t(const PagedKV &kv, const mlxcat_rope &rope, const RopeAppen
     const int64_t units = (int64_t)a.M * chunks;
     if (units > 0x3fffffff) return cudaErrorInvalidValue;
     const unsigned grid = (unsigned)std::min<int64_t>((units + WARPS - 1) / WARPS, wave / WARPS);
-    return launch_pdl(rope_append_kernel<TI, TO, D, PARTNER>, dim3(grid), dim3(RA_THREADS), 0, st, kv, rope, a, chunks, per);
+    if (((a.q ? a.n_heads : 0) % HPI) == 0 && kv.n_kv % HPI == 0)
+        return launch_pdl(rope_append_kernel<TI, TO, D, PARTNER, false>, dim3(grid), dim3(RA_THREADS), 0, st, kv, rope, a, chunks, per);
+    return launch_pdl(rope_append_kernel<TI, TO, D, PARTNER, true>, dim3(grid), dim3(RA_THREADS), 0, st, kv, rope, a, chunks, per);
 }
 
 template <typename TI, typename TO, int D>
