@@ -480,7 +480,9 @@ MLXCAT_API int mlxcat_op_paged_attention(const mlxcat_paged_kv *kv, const void *
  * page_size pages for every row r of the batch): those pages are read once for
  * all tokens, on the tensor cores.  prefix_len 0 is mlxcat_op_paged_attention,
  * and so is a call whose rows would together read at most 128 MB of the prefix
- * (L2 serves that faster than a second pass and a join). */
+ * (L2 serves that faster than a second pass and a join).  Where the prefix is
+ * read once, a NaN or infinite V entry of it can reach tokens that see only a
+ * part of the prefix (tpos < prefix_len - 1). */
 MLXCAT_API size_t mlxcat_op_shared_prefix_attention_workspace(int32_t M, int32_t qg, int32_t n_heads,
                                                               int32_t n_kv_heads, int32_t head_dim,
                                                               int32_t prefix_len);
@@ -499,7 +501,7 @@ MLXCAT_API int mlxcat_op_shared_prefix_attention(const mlxcat_paged_kv *kv, int3
  * nk.  A query that sees no key gets zeros; tokens outside the sequences are
  * left as they were.  out [Tq][n_heads][head_dim].  No sequence's values reach
  * another's; within a causal sequence a NaN or infinite V entry can reach
- * queries up to 127 positions before it.  n_heads / n_kv_heads <= 64.  *err
+ * queries up to 255 positions before it.  n_heads / n_kv_heads <= 64.  *err
  * (device int, may be NULL) becomes non-zero if a pipeline wait timed out. */
 MLXCAT_API int mlxcat_op_packed_attention(const void *q, const void *k, const void *v, int32_t dtype,
                                           int64_t q_stride, int64_t k_stride, int64_t v_stride, int32_t Tq,
