@@ -103,6 +103,7 @@ struct Args {
     const int32_t *trow, *tpos;
     int M, prefix_len, splits;
     float *o_part, *ml_part;
+    unsigned long long *ready, token;   // the sign for the kernel beside the pass
     int Hq, Hkv, G, TQ;         // TQ tokens of G rows each fill a tile
     float scale_log2;
     void *out;
@@ -324,8 +325,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     tc::fence_after_sync();
     const uint32_t tmem = fb.tmem;
     // the kernel that follows a prefix pass starts on the SMs that this one leaves
-    // free, without waiting for it: so the pass's own predecessor must be done first
+    // free, without waiting for it: so the pass's own predecessor must be done first,
+    // and the pass hands on, by a release, that it has seen that
     griddep_wait();
+    if (a.prefix && blockIdx.x == 0 && threadIdx.x == 0) tc::st_release_gpu(a.ready, a.token);
     griddep_launch_dependents();
 
     // The next item of a reading warp (all but the producer): its number, then what
@@ -795,7 +798,7 @@ int prefix_max_splits(int M, int n_heads, int n_kv, int prefix_len, int sm_count
 cudaError_t prefix_attn(const PagedKV &kv, const PagedQuery &q, int prefix_len, const PrefixPartials &part, cudaStream_t st) {
     Args a = {};
     a.prefix = 1; a.kv = kv; a.trow = q.trow; a.tpos = q.tpos; a.M = q.M; a.prefix_len = prefix_len; a.splits = part.splits;
-    a.o_part = part.o; a.ml_part = part.ml;
+    a.o_part = part.o; a.ml_part = part.ml; a.ready = part.ready; a.token = part.token;
     a.Hq = q.n_heads; a.Hkv = kv.n_kv; a.G = q.n_heads / kv.n_kv; a.TQ = TM / a.G;
     a.scale_log2 = q.scale_log2; a.err = q.err;
     CUtensorMap qm, km, vm;

@@ -58,9 +58,12 @@ struct PagedQuery {
 };
 
 // Partials of a shared-prefix pass: fp32 sums [splits][n_kv][D / 8][M * G rows][8]
-// and (max, sum) pairs [splits][n_kv][M * G].
+// and (max, sum) pairs [splits][n_kv][M * G].  *ready: `token` (a new one each
+// call) once the pass has waited for all that was launched before it, 0 again
+// after the call.
 struct PrefixPartials {
     float *o = nullptr, *ml = nullptr;
+    unsigned long long *ready = nullptr, token = 0;
     int splits = 0, ctas = 0;   // CTAs of the pass
 };
 

@@ -1,7 +1,10 @@
 // paged_api.cu -- entry points of the paged-cache operators (include/mlxcat_cuda.h):
 // checks of the arguments, then the launches of rope.cu, paged_attn.cu and
-// fa_packed.cu.  Nothing is allocated, read back or kept between calls.
+// fa_packed.cu.  Nothing is allocated, read back or kept between calls, but for the
+// count of calls that fresh_token takes its values from.
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <cmath>
 
 #include "../../include/mlxcat_cuda.h"
@@ -79,7 +82,7 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct PrefixLayout {
     int splits;
-    size_t ml_at, bytes;
+    size_t ml_at, ready_at, bytes;
 };
 PrefixLayout prefix_layout(int M, int n_heads, int n_kv, int D, int prefix_len) {
     PrefixLayout p;
@@ -87,8 +90,25 @@ PrefixLayout prefix_layout(int M, int n_heads, int n_kv, int D, int prefix_len) 
     p.splits = prefix_max_splits(M, n_heads, n_kv, prefix_len, SM_MAX);
     const size_t rows = (size_t)p.splits * M * n_heads;   // n_kv * (M * G)
     p.ml_at = up256(rows * D * 4);
-    p.bytes = p.ml_at + up256(rows * 8);
+    p.ready_at = p.ml_at + up256(rows * 8);
+    p.bytes = p.ready_at + up256(sizeof(unsigned long long));
     return p;
+}
+
+// What a shared-prefix call writes as its sign in the workspace: the workspace may
+// hold anything, so 64 bits that no other call of this process writes and that
+// stray contents match with probability 2^-64 (a bijection of a counter: the
+// finaliser of SplitMix64, Steele, Lea and Flood, OOPSLA 2014).  Never 0.
+unsigned long long fresh_token() {
+    static const uint64_t seed = (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() << 20;
+    static std::atomic<uint64_t> calls{0};
+    for (;;) {
+        uint64_t z = (seed + calls.fetch_add(1, std::memory_order_relaxed)) * 0x9E3779B97F4A7C15ull;
+        z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+        z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+        z ^= z >> 31;
+        if (z) return z;
+    }
 }
 
 int query_of(const mlxcat_paged_kv *c, const void *q, int32_t M, int32_t qg, int32_t n_heads, float scale,
@@ -254,6 +274,8 @@ int mlxcat_op_shared_prefix_attention(const mlxcat_paged_kv *c, int32_t prefix_l
         char *at = static_cast<char *>(workspace) + own;
         pre.o = reinterpret_cast<float *>(at);
         pre.ml = reinterpret_cast<float *>(at + l.ml_at);
+        pre.ready = reinterpret_cast<unsigned long long *>(at + l.ready_at);
+        pre.token = fresh_token();
         pre.splits = std::min(l.splits, prefix_splits(M, n_heads, kv.n_kv, prefix_len, std::min(sms, SM_MAX)));
         pre.ctas = (int)std::min<int64_t>((int64_t)pre.splits * prefix_items(M, n_heads, kv.n_kv), 0x7fffffff);
         const cudaError_t e = prefix_attn(kv, pq, prefix_len, pre, st);

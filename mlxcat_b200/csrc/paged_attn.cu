@@ -100,6 +100,10 @@ __device__ __forceinline__ void cpa16(uint32_t s, const void *g, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(g), "r"(bytes) : "memory");
 }
 
+// Tokens' rows and positions and page ids: plain loads, since an acquire orders
+// them and does not order loads by the read-only path.
+__device__ __forceinline__ int load_id(const int32_t *p) { return *p; }
+
 // What a group of tokens sees: its row and one past its last key.
 struct Group {
     int row, kend;
@@ -119,7 +123,7 @@ __device__ __forceinline__ Group group_alone(const PagedKV &kv, const PagedQuery
     Group x = {-1, 0};
 #pragma unroll 4
     for (int j = 0; j < n; ++j) {
-        const int r = __ldg(a.trow + t0 + j), p = __ldg(a.tpos + t0 + j);
+        const int r = load_id(a.trow + t0 + j), p = load_id(a.tpos + t0 + j);
         if (r >= 0) {
             x.row = max(x.row, r);
             x.kend = max(x.kend, p == 0x7fffffff ? p : p + 1);
@@ -156,6 +160,7 @@ struct PagedShape {
     static constexpr int MERGE_AT = EARLY ? RING : 0;
     static constexpr int SMEM = BODY + TAIL;
 };
+constexpr int NOBODY = 0x7fffffff;   // key limit of query rows that are padding or behind the group
 constexpr int MAX_GROUPS = 256;   // groups whose (row, last key) a CTA keeps
 
 // 8 features of a query row on their way through partials.
@@ -224,9 +229,10 @@ __device__ __forceinline__ void join_item(const PagedKV &kv, const PagedQuery &a
             }
         }
     };
+    // asked before the pieces are gathered, so that the load is not one more in the chain
+    auto padding = [&](int w) { return load_id(a.trow + t0 + (qt * QR + w / (D / 8)) / G) < 0; };
     auto write = [&](int w, const Joined &j) {
         const int r = w / (D / 8), d = (w % (D / 8)) * 8, rr = qt * QR + r, m = t0 + rr / G;
-        if (__ldg(a.trow + m) < 0) return;
         const float inv = j.l != 0.f ? 1.f / j.l : 0.f;
         uint4 y;
         y.x = Half2<T>::pack(j.acc[0] * inv, j.acc[1] * inv);
@@ -239,13 +245,15 @@ __device__ __forceinline__ void join_item(const PagedKV &kv, const PagedQuery &a
     if (P <= 1) {
         for (int w = threadIdx.x; w < W; w += blockDim.x) {
             Joined j;
+            const bool pad = padding(w);
             gather(w, 0, 1, j);
-            write(w, j);
+            if (!pad) write(w, j);
         }
         return;
     }
     const int g = threadIdx.x / W, w = threadIdx.x % W;
     Joined j;
+    const bool pad = g || padding(w);
     if (g < P) gather(w, g, P, j);
     float *mine = sm + threadIdx.x;
     const int bs = blockDim.x;
@@ -254,7 +262,7 @@ __device__ __forceinline__ void join_item(const PagedKV &kv, const PagedQuery &a
 #pragma unroll
     for (int i = 0; i < 8; ++i) mine[(2 + i) * bs] = j.acc[i];
     __syncthreads();
-    if (g == 0) {
+    if (!pad) {
         float mx = j.mx;
         for (int p = 1; p < P; ++p) mx = fmaxf(mx, sm[p * W + w]);
         Joined t;
@@ -277,6 +285,7 @@ attn_join(const PagedKV kv, const PagedQuery a, int QR, const float *__restrict_
     __shared__ float sm[10 * 256];
     griddep_launch_dependents();
     griddep_wait();
+    if (pre.splits && blockIdx.x == 0 && threadIdx.x == 0) *pre.ready = 0;   // for a replay of this call
     join_item<T, D>(kv, a, QR, blockIdx.x, o_part, ml_part, meta[blockIdx.x], pre, sm);
 }
 
@@ -311,9 +320,18 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
 
     // Behind a prefix pass this kernel needs nothing of it: it starts on the SMs the
     // pass leaves free (which itself lets it start only once all before the pass is
-    // done) and waits at its end, so that the join after it waits for both.
+    // done) and waits at its end, so that the join after it waits for both.  That what
+    // was written before the pass is visible here does not follow from the early start:
+    // the pass releases its sign once it has waited for those writes, and this kernel
+    // acquires it.  A CTA that does not find the sign yet waits for the pass (all of
+    // them waiting at once: 64 tokens over an 8k document 42 -> 65 us).
     griddep_launch_dependents();
-    if (!force_partial) griddep_wait();
+    bool ordered = false;
+    if (force_partial) {
+        if (threadIdx.x == 0) ordered = tc::ld_acquire_gpu(pre.ready) == pre.token;
+        ordered = __syncthreads_or(ordered);
+    }
+    if (!ordered) griddep_wait();
 
     // ---- where this CTA's stretch of units starts: thread x sums the groups of
     // its chunk, a scan gives the total and the chunk that holds the start
@@ -327,7 +345,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         __syncthreads();
 #pragma unroll 2
         for (int m = threadIdx.x; m < a.M; m += PT) {
-            const int r = __ldg(a.trow + m), p = __ldg(a.tpos + m), i = m / a.qg;
+            const int r = load_id(a.trow + m), p = load_id(a.tpos + m), i = m / a.qg;
             if (r >= 0) {
                 atomicMax(&info[i].row, r);
                 atomicMax(&info[i].kend, p == 0x7fffffff ? p : p + 1);
@@ -385,7 +403,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         if (force_partial) continue;
         const int t0 = i * a.qg, n = min(a.qg, a.M - t0);
         for (int j = 0; j < n; ++j) {
-            if (__ldg(a.trow + t0 + j) < 0) continue;   // padding stays as it was
+            if (load_id(a.trow + t0 + j) < 0) continue;   // padding stays as it was
             uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + (size_t)(t0 + j) * Hq * D);
             for (int x = lane; x < Hq * D / 8; x += 32) dst[x] = make_uint4(0, 0, 0, 0);
         }
@@ -448,7 +466,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
                 const int64_t key = (int64_t)p.kfirst + (int64_t)(s + lane) * UNIT + 8 * e;
                 int id = -1;
                 if (s + lane < p.steps && key < p.kend) {
-                    id = __ldg(p.table + (key >> kv.page_shift));
+                    id = load_id(p.table + (key >> kv.page_shift));
                     if (id < 0 || id >= kv.n_pages) {
                         id = -1;
                         if (a.err) atomicExch(a.err, PE_PAGE);
@@ -481,8 +499,9 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         }
         if (threadIdx.x < S::QR) {
             const int r = threadIdx.x, m = p.t0 + div_g(p.qt * S::QR + r);
-            // rows nobody reads see everything: they need no mask
-            lim_s[r] = r < p.nq && __ldg(a.trow + m) >= 0 ? __ldg(a.tpos + m) : 0x7fffffff;
+            // rows nobody reads see everything: they need no mask (no position is beyond NOBODY - 1:
+            // the table ends before it)
+            lim_s[r] = r < p.nq && load_id(a.trow + m) >= 0 ? min(load_id(a.tpos + m), NOBODY - 1) : NOBODY;
         }
 #pragma unroll
         for (int s = 0; s < ST - 1; ++s) {
@@ -512,7 +531,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         // query rows as B operands, key limits of this lane's columns
         uint32_t qf[NT][D / 16][2];
         int lim[NT][2];
-        int lim_min = 0x7fffffff;
+        int lim_min = NOBODY;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = nt * 8 + (lane & 7);
@@ -689,7 +708,9 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
             const float inv0 = l[0] != 0.f ? 1.f / l[0] : 0.f, inv1 = l[1] != 0.f ? 1.f / l[1] : 0.f;
             // 16-bit results go out as pairs of features: even g the first row's, odd g the second's
             const int rw = ra + (g & 1), rr = qt * S::QR + rw, j = div_g(rr), m = t0 + j;
-            const bool write = rw < nq && (!direct || __ldg(a.trow + m) >= 0);
+            // (without EARLY the limits in shared memory are still this piece's)
+            const int own = !S::EARLY ? lim_s[rw] : (g & 1) ? lim[nt][1] : lim[nt][0];
+            const bool write = rw < nq && (!direct || own != NOBODY);
             T *dst = reinterpret_cast<T *>(a.out) + ((size_t)m * Hq + h * G + rr - j * G) * D + (g & ~1);
 #pragma unroll
             for (int mt = 0; mt < S::MT; ++mt) {
@@ -730,6 +751,7 @@ paged_attn_kernel(const PagedKV kv, const PagedQuery a, int key_begin, int force
         // a call of few units is one cluster: it joins its pieces itself, behind a
         // barrier that also orders their stores
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        if (force_partial && blockIdx.x == 0 && threadIdx.x == 0) *pre.ready = 0;   // for a replay of this call
         for (size_t i = blockIdx.x; i < (size_t)items; i += gridDim.x) join_item<T, D>(kv, a, S::QR, i, o_part, ml_part, meta[i], pre, reinterpret_cast<float *>(psm));
     }
 }

@@ -752,3 +752,102 @@ def test_serving_run(dt, d):
             loose(o1[s], qq, keys[r], vals[r], tpos[s].long())
             loose(o2[s], qq, keys[r], vals[r], tpos[s].long())
             at[r] += qg
+
+
+# ------------------------------------------------- shared prefix read once, every token against the formula
+class Once:
+    """Rows behind one prefix with at most a page of own keys each, so that the formula takes all tokens in
+    one go; keys no token sees are NaN.  Tokens come in groups of qg, the last ones of their row."""
+
+    def __init__(self, h, hk, d, dt, qg, ps, prefix, rows, seed=0):
+        self.h, self.hk, self.d, self.dt, self.qg, self.ps, self.prefix, self.rows = h, hk, d, dt, qg, ps, prefix, rows
+        g = gen(seed + h + rows)
+        own = [qg + r % (ps - qg + 1) for r in range(rows)]
+        table, n_pages = tables([prefix + n for n in own], ps, seed=seed, lead=(0,) * (prefix // ps))
+        self.cache = Paged(hk, d, ps, n_pages, dt, table)
+        self.cache.put(0, rnd((prefix, hk, d), g, dt), rnd((prefix, hk, d), g, dt))
+        for r, n in enumerate(own):
+            self.cache.put(r, rnd((n, hk, d), g, dt), rnd((n, hk, d), g, dt), prefix)
+        self.trow = ints([r for r in range(rows) for _ in range(qg)])
+        self.tpos = ints([prefix + n - qg + j for n in own for j in range(qg)])
+        self.q = rnd((rows * qg, h, d), g, dt)
+        assert rows * prefix * hk * d * 4 > 128 << 20        # read once
+
+    def run(self, ws=None, err=None):
+        out = torch.full_like(self.q, 9.0)
+        A.check(paged(self.cache, self.q, self.qg, self.trow, self.tpos, out, self.prefix, ws=ws, err=err))
+        return out
+
+    def check(self, out, sees=None):
+        """sees: tokens that see keys at all (default: those of a row, at a position >= 0)."""
+        c, g = self.cache, self.h // self.hk
+        live = (self.trow >= 0) & (self.tpos >= 0) if sees is None else sees
+        assert (out[self.trow < 0] == 9.0).all()
+        assert (out[(self.trow >= 0) & ~live] == 0).all()
+        at = live.nonzero()[:, 0]
+        row, pos = self.trow[at].long(), self.tpos[at].long()
+        q = self.q[at].double().view(len(at), self.hk, g, self.d)
+        kp, vp = (x.double() for x in c.row(0, self.prefix))
+        page = c.table[row, self.prefix // self.ps].long()
+        ko, vo = (x[page].double() for x in (c.view(c.k), c.view(c.v)))       # [token][kv head][key][d]
+        seen = torch.arange(self.prefix + self.ps, device="cuda")[None, :] <= pos[:, None]
+        own_seen = seen[:, None, self.prefix:, None]
+        ko, vo = ko.masked_fill(~own_seen, 0.0), vo.masked_fill(~own_seen, 0.0)
+        s = torch.cat([torch.einsum("nkgd,pkd->nkgp", q, kp), torch.einsum("nkgd,nkpd->nkgp", q, ko)], -1) / math.sqrt(self.d)
+        s = s.masked_fill(~seen[:, None, None, :], float("-inf"))
+        e = torch.exp(s - s.amax(-1, keepdim=True))
+        tot = e.sum(-1, keepdim=True)
+        w = e / tot
+        wp, wo = w[..., :self.prefix], w[..., self.prefix:]
+        y = torch.einsum("nkgp,pkd->nkgd", wp, vp) + torch.einsum("nkgp,nkpd->nkgd", wo, vo)
+        a = torch.einsum("nkgp,pkd->nkgd", wp, vp.abs()) + torch.einsum("nkgp,nkpd->nkgd", wo, vo.abs())
+        err = 2 * self.d * 2.0 ** -24 * q.norm(dim=-1).max() * max(kp.norm(dim=-1).max(), ko.norm(dim=-1).max()) / math.sqrt(self.d)
+        u = half_step(self.dt)
+        tol = u * y.abs() + 2 * a * (u + err + 2.0 ** -21) + 1e-7
+        if self.dt == "f16":
+            tol = tol + s.shape[-1] * 2.0 ** -25 * max(vp.abs().max(), vo.abs().max()) / tot
+        got = out[at].double().view_as(y)
+        assert torch.isfinite(got).all()
+        worst = ((got - y).abs() / tol).flatten(1).amax(1)
+        assert worst.max().item() <= 1.0, (worst.max().item(), at[worst > 1.0][:20].tolist(), int((worst > 1.0).sum()))
+
+
+def test_shared_prefix_after_append_replayed():
+    """Keys, queries, positions and page ids written right before the call, captured and replayed: the pass over
+    the prefix and the kernel beside it both see them, whatever the workspace held."""
+    qg, ps, prefix, rows, h, hk, d = 2, 64, 2048, 70, 32, 8, 128
+    x = Once(h, hk, d, "f16", qg, ps, prefix, rows)
+    for c in (x.cache.k, x.cache.v):
+        c.nan_to_num_(nan=0.5)                       # a row's page is full
+    m, g, cg = rows * qg, gen(31), torch.Generator().manual_seed(31)
+    xin = torch.zeros((m, (h + 2 * hk) * d), device="cuda")
+    table, tpos = x.cache.table.clone(), x.tpos.clone()
+    out = torch.zeros((m, h, d), dtype=torch.float16, device="cuda")
+    ws = torch.empty(L.mlxcat_op_shared_prefix_attention_workspace(m, qg, h, hk, d, prefix), dtype=torch.uint8, device="cuda")
+
+    def step():
+        x.cache.table.copy_(table)
+        x.tpos.copy_(tpos)
+        A.check(append(x.cache, None, xin[:, :h * d], xin[:, h * d:(h + hk) * d], xin[:, (h + hk) * d:], "f32", x.trow, x.tpos, x.q))
+        A.check(paged(x.cache, x.q, qg, x.trow, x.tpos, out, prefix, ws=ws))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(12):
+        xin.copy_(torch.randn(xin.shape, device="cuda", generator=g))
+        first = prefix + torch.randint(0, ps - qg + 1, (rows,), generator=cg)
+        tpos.copy_((first[:, None] + torch.arange(qg)).flatten())
+        table.copy_(table[torch.randperm(rows, generator=cg).cuda()])        # rows change their own pages
+        if i % 3 == 0:
+            ws.fill_(0xff)
+        if i % 3 == 1:
+            ws.random_(generator=g)
+        graph.replay() if i % 4 else step()
+        torch.cuda.synchronize()
+        x.check(out)
