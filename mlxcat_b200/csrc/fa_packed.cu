@@ -657,6 +657,9 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             const float inv = l != 0.f ? 1.f / l : 0.f;
             T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(w.tok0 + tk) * a.Hq + w.h * a.G + gh) * D;
             const size_t part_rows = (size_t)a.M * a.G, part_row = (size_t)(w.tok0 + tk) * a.G + gh;
+            const size_t part = (size_t)w.split * a.Hkv + w.h;
+            // behind this arrival the producer may write the item after next into w: nothing
+            // reads w below
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(tc::smem_u32(&fb.work_free[it & 1]));
 #pragma unroll 1
@@ -678,7 +681,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     if (!live) acc[x] = 0u;
                 if (!pad && a.prefix) {
                     // [split][KV head][8 features][row][8]: a warp's 32 rows are one kilobyte
-                    float *p = a.o_part + (((size_t)w.split * a.Hkv + w.h) * (D / 8) + c * 4) * part_rows * 8 + part_row * 8;
+                    float *p = a.o_part + (part * (D / 8) + c * 4) * part_rows * 8 + part_row * 8;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) store32(p + x * part_rows * 8, acc + x * 8);
                 } else if (!pad) {
@@ -697,7 +700,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 }
             }
             if (a.prefix && !pad)
-                *reinterpret_cast<float2 *>(a.ml_part + (((size_t)w.split * a.Hkv + w.h) * part_rows + part_row) * 2) = make_float2(m_used, l);
+                *reinterpret_cast<float2 *>(a.ml_part + (part * part_rows + part_row) * 2) = make_float2(m_used, l);
         }
     }
     tc::fence_before_sync();

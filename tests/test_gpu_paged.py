@@ -851,3 +851,27 @@ def test_shared_prefix_after_append_replayed():
         graph.replay() if i % 4 else step()
         torch.cuda.synchronize()
         x.check(out)
+
+
+def once_items(h, hk, m):
+    """(pair of tiles, KV head) items of the pass over the prefix: two tiles of 128 (token, head) rows each."""
+    return -(-m // (2 * (128 // (h // hk)))) * hk
+
+
+@pytest.mark.parametrize("h,hk,d,dt,qg,ps,prefix,rows", [
+    (64, 8, 128, "f16", 8, 64, 256, 300),       # two key blocks, 600 items
+    (32, 8, 128, "bf16", 5, 128, 128, 960),     # one key block, 600 items
+    (32, 16, 64, "f16", 4, 8, 1160, 650),       # ten blocks, the last of 8 keys
+    (8, 8, 128, "bf16", 1, 16, 272, 11000)])    # one head a group, many rows of one token
+def test_shared_prefix_many_items_a_cta(h, hk, d, dt, qg, ps, prefix, rows):
+    """A CTA of the pass takes three items and more: descriptors, queries and O change hands, every token is right."""
+    x = Once(h, hk, d, dt, qg, ps, prefix, rows)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert once_items(h, hk, rows * qg) > 2 * sms
+    err = ints([0])
+    out = x.run(err=err)
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    x.check(out)
+    for _ in range(5):
+        assert torch.equal(out, x.run())
