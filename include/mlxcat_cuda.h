@@ -384,9 +384,9 @@ MLXCAT_API int mlxcat_op_gemm_f16(const uint16_t *w, int32_t N, int32_t K, const
  * positions, attention of single tokens and verify groups, the same for a batch
  * whose first blocks are shared, and the causal attention of several prompts at
  * once.  All take device pointers and a stream of the current device, use no
- * memory but their arguments' (each call its own workspace: calls whose kernels
- * may overlap must not share one), read no device value on the host and can be
- * captured in a graph.
+ * memory but their arguments' (each call its own workspace, 16-byte aligned:
+ * calls whose kernels may overlap must not share one), read no device value on
+ * the host and can be captured in a graph.
  *
  * Element types: the cache, queries and outputs are fp16 or bf16 (one type per
  * call); rope_append also reads fp32 (a projection's accumulator). */

@@ -80,6 +80,7 @@ bool attention_shape(int32_t M, int32_t qg, int32_t n_heads, int32_t n_kv, int32
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+constexpr uintptr_t PARTIALS_ALIGN = 32;
 struct PrefixLayout {
     int splits;
     size_t ml_at, ready_at, bytes;
@@ -91,7 +92,9 @@ PrefixLayout prefix_layout(int M, int n_heads, int n_kv, int D, int prefix_len) 
     const size_t rows = (size_t)p.splits * M * n_heads;   // n_kv * (M * G)
     p.ml_at = up256(rows * D * 4);
     p.ready_at = p.ml_at + up256(rows * 8);
-    p.bytes = p.ready_at + up256(sizeof(unsigned long long));
+    // the pass stores its sums 32 bytes at a time: room to start on such a boundary in
+    // a workspace that itself starts on one of 16
+    p.bytes = p.ready_at + up256(sizeof(unsigned long long) + PARTIALS_ALIGN - 16);
     return p;
 }
 
@@ -271,7 +274,7 @@ int mlxcat_op_shared_prefix_attention(const mlxcat_paged_kv *c, int32_t prefix_l
     if (apart <= ((int64_t)128 << 20)) prefix_len = 0;
     if (prefix_len) {
         const PrefixLayout l = prefix_layout(M, n_heads, kv.n_kv, kv.D, prefix_len);
-        char *at = static_cast<char *>(workspace) + own;
+        char *at = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(workspace) + own + PARTIALS_ALIGN - 1) & ~(PARTIALS_ALIGN - 1));
         pre.o = reinterpret_cast<float *>(at);
         pre.ml = reinterpret_cast<float *>(at + l.ml_at);
         pre.ready = reinterpret_cast<unsigned long long *>(at + l.ready_at);

@@ -875,3 +875,27 @@ def test_shared_prefix_many_items_a_cta(h, hk, d, dt, qg, ps, prefix, rows):
     x.check(out)
     for _ in range(5):
         assert torch.equal(out, x.run())
+
+
+@pytest.mark.parametrize("once", [True, False])
+def test_workspace_on_any_16_byte_boundary(once):
+    """A workspace cut from an arena: 16-byte aligned is enough, nothing outside it is written."""
+    x = Once(32, 8, 128, "bf16", 1, 64, 2048, 70)
+    n = 70 if once else 9                                    # 9 rows read the prefix one by one
+    q, trow, tpos = x.q[:n], x.trow[:n], x.tpos[:n]
+    assert (n * x.prefix * x.hk * x.d * 4 > 128 << 20) == once
+    size = L.mlxcat_op_shared_prefix_attention_workspace(n, 1, x.h, x.hk, x.d, x.prefix)
+    arena, outs = torch.empty(size + 256, dtype=torch.uint8, device="cuda"), []
+    for at in (0, 16, 32, 48, 112):
+        arena.fill_(0xab)
+        ws = arena[at:at + size]
+        assert ws.data_ptr() % 256 == at
+        outs.append(torch.full_like(q, 9.0))
+        A.check(paged(x.cache, q, 1, trow, tpos, outs[-1], x.prefix, ws=ws))
+        torch.cuda.synchronize()
+        assert (arena[:at] == 0xab).all() and (arena[at + size:] == 0xab).all()
+    assert all(torch.equal(outs[0], o) for o in outs)
+    if once:
+        x.check(outs[1])
+    else:
+        check_rows(x.cache, q, 1, trow, tpos, outs[1], "bf16")
