@@ -464,9 +464,9 @@ MLXCAT_API int mlxcat_op_rope_append(const mlxcat_paged_kv *kv, const mlxcat_rop
  * tokens, k + 1: a verify step; a group may end in padding tokens, trow < 0).
  * q, out [M][n_heads][head_dim] in the cache's type; scale 0: 1 / sqrt(head_dim).
  * A token that sees no key (tpos < 0) gets zeros, a padding token's output is
- * left as it was.  A row or position outside the table sets *err (device int,
- * may be NULL) and is cut to the table; a page id outside the cache sets it and
- * reads as zeros.  Keys past a group's last position are not read; a NaN or
+ * left as it was.  A row outside the table sets *err (device int, may be NULL)
+ * and its tokens get zeros; a position outside sets it and is cut to the table; a
+ * page id outside the cache sets it and reads as zeros.  Keys past a group's last position are not read; a NaN or
  * infinite V entry reaches every token of a group that may see it. */
 MLXCAT_API size_t mlxcat_op_paged_attention_workspace(int32_t M, int32_t qg, int32_t n_heads, int32_t n_kv_heads,
                                                       int32_t head_dim);

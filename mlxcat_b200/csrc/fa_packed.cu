@@ -580,8 +580,11 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             bool pad = !valid;
             if (valid) {
                 if (!a.prefix) lim = a.causal ? min(w.first_lim + tk, w.kend - 1) : w.kend - 1;
-                else if (__ldg(a.trow + w.tok0 + tk) >= 0) lim = min(__ldg(a.tpos + w.tok0 + tk), w.kend - 1);
-                else pad = true;
+                else {
+                    const int row = __ldg(a.trow + w.tok0 + tk), pos = __ldg(a.tpos + w.tok0 + tk);
+                    pad = row < 0;
+                    if (row < a.kv.rows) lim = min(pos, w.kend - 1);   // a row outside the table sees nothing
+                }
             }
             lim = pad ? 0x3fffffff : lim - w.kbeg;   // rows nobody reads need no mask
             const int ns = w.ns;

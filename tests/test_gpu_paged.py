@@ -785,6 +785,8 @@ class Once:
         assert (out[self.trow < 0] == 9.0).all()
         assert (out[(self.trow >= 0) & ~live] == 0).all()
         at = live.nonzero()[:, 0]
+        if not len(at):
+            return
         row, pos = self.trow[at].long(), self.tpos[at].long()
         q = self.q[at].double().view(len(at), self.hk, g, self.d)
         kp, vp = (x.double() for x in c.row(0, self.prefix))
@@ -899,3 +901,48 @@ def test_workspace_on_any_16_byte_boundary(once):
         x.check(outs[1])
     else:
         check_rows(x.cache, q, 1, trow, tpos, outs[1], "bf16")
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_shared_prefix_read_once_empty_padding_and_out_of_range(dt):
+    """Read once or row by row, the call says the same: tokens of a row outside the table and tokens before
+    position 0 get zeros, padding stays, positions past the table are cut to it, the flag tells."""
+    qg, rows = 3, 70
+    x = Once(32, 8, 128, dt, qg, 64, 2048, rows)
+    for c in (x.cache.k, x.cache.v):
+        c.nan_to_num_(nan=0.5)                                # whole own pages, for the cut positions
+    cap = x.prefix + x.ps
+    x.q, x.trow, x.tpos = x.q[:-2].contiguous(), x.trow[:-2].contiguous(), x.tpos[:-2].contiguous()   # a short last group
+    def group(i):
+        return slice(i * qg, (i + 1) * qg)
+    x.trow[group(0)] = -1                                     # padding first
+    x.tpos[group(1)] = -1                                     # no key
+    x.tpos[group(2)] = ints([-2, -1, 0])                      # a key for the last of the group
+    x.trow[6 * qg + 1:7 * qg] = -1                            # a group that ends in padding
+    x.tpos[group(7)] = ints([x.prefix - 2, x.prefix - 1, x.prefix])
+    x.tpos[group(8)] = ints([5, 6, 7])
+    err = ints([0])
+    x.check(x.run(err=err))
+    assert err.item() == 0
+    outside = [(3, rows), (4, rows + 1), (9, 2 ** 31 - 1)]
+    for bad in (outside, outside + [(1, rows)], [(i, rows + i) for i in range(rows)]):
+        keep = x.trow.clone()
+        for i, r in bad:
+            x.trow[group(i)] = r
+        err.zero_()
+        out = x.run(err=err)
+        assert err.item() == 51
+        x.check(out, (x.trow >= 0) & (x.trow < rows) & (x.tpos >= 0))
+        few = slice(0, 10 * qg)                               # the same tokens row by row
+        assert 10 * x.prefix * x.hk * x.d * 4 <= 128 << 20
+        apart = torch.full_like(x.q[few], 9.0)
+        A.check(paged(x.cache, x.q[few], qg, x.trow[few], x.tpos[few], apart, x.prefix))
+        none = (x.trow[few] < 0) | (x.trow[few] >= rows) | (x.tpos[few] < 0)
+        assert torch.equal(apart[none], out[few][none])
+        x.trow = keep
+    x.tpos[group(5)] = ints([cap - 1, cap, 2 ** 31 - 1])
+    err.zero_()
+    out = x.run(err=err)
+    assert err.item() == 52
+    x.tpos[group(5)] = cap - 1
+    x.check(out)
