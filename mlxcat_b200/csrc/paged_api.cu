@@ -40,8 +40,10 @@ int paged_kv(const mlxcat_paged_kv *c, PagedKV *out) {
         if (x.stride <= 0 || x.stride % 8 || x.stride > ((int64_t)1 << 38))
             return op_error(MLXCAT_E_INVALID, "paged cache: strides must be positive multiples of 8 elements");
         if (x.count > 1 && x.stride < extent) return op_error(MLXCAT_E_INVALID, "paged cache: strides overlap");
+        // extent + stride * (count - 1) <= 2^60, without a product that could wrap
+        if (x.count > 1 && (((int64_t)1 << 60) - extent) / x.stride < x.count - 1)
+            return op_error(MLXCAT_E_INVALID, "paged cache: extent too large");
         extent += x.stride * (x.count - 1);
-        if (extent > ((int64_t)1 << 60)) return op_error(MLXCAT_E_INVALID, "paged cache: extent too large");
     }
     PagedKV kv;
     kv.k = c->k; kv.v = c->v; kv.table = c->page_table;

@@ -184,3 +184,13 @@ def test_structs_match_the_header(tmp_path):
     for ln in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines():
         cname, key, val = ln.split()
         assert int(val) == (C.sizeof(structs[cname]) if key == "size" else getattr(structs[cname], key).offset), ln
+
+
+@pytest.mark.parametrize("change", [
+    dict(page_stride=1 << 38, n_pages=(1 << 26) + 1), dict(page_stride=1 << 38, n_pages=2 ** 31 - 1),
+    dict(page_stride=1 << 37, n_pages=(1 << 25) + 1, head_stride=1 << 33),
+    dict(head_stride=1 << 38, n_kv_heads=1 << 26, page_stride=2048, page_size=16)], ids=str)
+def test_cache_extent_past_64_bits_refused(change):
+    """Strides times counts past 2^63 elements: the sum that finds them too large must not wrap."""
+    assert append(kv(**change)) == A.E_INVALID
+    assert paged(kv(**change), heads=change.get("n_kv_heads", 8)) == A.E_INVALID
