@@ -451,7 +451,9 @@ MLXCAT_API int mlxcat_rope_init(mlxcat_rope *rope, int32_t rotary_dim, int32_t l
  * q and q_out may both be NULL (append only).  A token with trow < 0 is padding:
  * nothing is written for it.  A row, position or page outside the table or the
  * cache sets *err (device int, may be NULL) and its key and value are not
- * written.  Two tokens with the same row and position leave one of the two. */
+ * written.  Tokens of one call have places of their own: of two with the same row
+ * and position every 16 bytes of the key and the value are one token's, and not
+ * all need be the same one's. */
 MLXCAT_API int mlxcat_op_rope_append(const mlxcat_paged_kv *kv, const mlxcat_rope *rope, const void *q,
                                      const void *k, const void *v, int32_t in_dtype, int64_t q_stride,
                                      int64_t k_stride, int64_t v_stride, int32_t M, int32_t n_heads,

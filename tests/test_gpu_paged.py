@@ -946,3 +946,20 @@ def test_shared_prefix_read_once_empty_padding_and_out_of_range(dt):
     assert err.item() == 52
     x.tpos[group(5)] = cap - 1
     x.check(out)
+
+
+def test_append_same_place_twice():
+    """Tokens that share a place: every 16 bytes there are one of the tokens', the queries are each its own."""
+    h, hk, d, n = 8, 8, 128, 64
+    cache = Paged(hk, d, 16, 2, "f16", ints([[0, 1]]), fill=9.0)
+    x = rnd((n, (h + 2 * hk) * d), gen(5), "f16")
+    q, k, v = x[:, :h * d], x[:, h * d:(h + hk) * d], x[:, (h + hk) * d:]
+    q_out = torch.zeros((n, h, d), dtype=torch.float16, device="cuda")
+    A.check(append(cache, None, q, k, v, "f16", ints([0] * n), ints([5] * (n - 1) + [17]), q_out))
+    assert torch.equal(q_out.view(n, -1), q)
+    for c, src in ((cache.k, k), (cache.v, v)):
+        got = c[0, :, 5].reshape(-1, 8)
+        assert (got[None] == src[:-1].reshape(n - 1, -1, 8)).all(-1).any(0).all()
+        assert torch.equal(c[1, :, 1].reshape(-1), src[-1])
+        c[0, :, 5] = c[1, :, 1] = 9.0
+        assert (c == 9.0).all()
