@@ -963,3 +963,106 @@ def test_append_same_place_twice():
         assert torch.equal(c[1, :, 1].reshape(-1), src[-1])
         c[0, :, 5] = c[1, :, 1] = 9.0
         assert (c == 9.0).all()
+
+
+# ------------------------------------------------------------------------------------------ more of the range
+@pytest.mark.parametrize("d,rd,layout,src,dt", [(128, 96, 0, "f32", "f16"), (128, 72, 0, "bf16", "bf16"), (64, 48, 0, "f16", "bf16"),
+                                                (128, 96, 1, "f16", "f16"), (64, 32, 0, "f32", "f16"), (128, 64, 0, "bf16", "f16")])
+def test_append_rotary_widths(d, rd, layout, src, dt):
+    """Rotary widths between half a head and a head, and those whose partner is another lane's."""
+    test_append(d, 6, 2, dt, src, rd, layout, 0, True, 16, False, 21)
+
+
+@pytest.mark.parametrize("keys", [8, 64, 72, 130, 192, 200, 320, 384, 3904, 3912])
+def test_paged_attention_every_cluster_size(keys):
+    """One row, one KV head, tables of 1 to 62 units: one cluster of 4 to 8 CTAs, then two kernels."""
+    g, ps = gen(keys), 8
+    table, n_pages = tables([keys], ps, spare=0)
+    cache = Paged(1, 64, ps, n_pages, "bf16", table)
+    fill_rows(cache, [keys], g, "bf16")
+    for n in {1, keys // 2, keys}:
+        q = rnd((1, 5, 64), g, "bf16")
+        out = torch.full_like(q, 9.0)
+        A.check(paged(cache, q, 1, ints([0]), ints([n - 1]), out))
+        check_rows(cache, q, 1, ints([0]), ints([n - 1]), out, "bf16")
+
+
+@pytest.mark.parametrize("width", [0, 500])
+def test_shared_prefix_without_own_keys(width):
+    """The prefix is all there is: a table that ends with it, and one with empty pages behind it."""
+    rows, h, hk, d, ps, prefix, dt = 70, 32, 8, 128, 64, 2048, "f16"
+    table, n_pages = tables([prefix] * rows, ps, lead=(0,) * (prefix // ps))
+    table = torch.cat([table[:, :prefix // ps], torch.full((rows, width), -1, dtype=torch.int32, device="cuda")], 1).contiguous()
+    cache, g = Paged(hk, d, ps, n_pages, dt, table), gen(3)
+    cache.put(0, rnd((prefix, hk, d), g, dt), rnd((prefix, hk, d), g, dt))
+    q, trow = rnd((rows, h, d), g, dt), ints(list(range(rows)))
+    tpos = ints([prefix - 1 if r % 3 else r * 29 for r in range(rows)])
+    out, err = torch.full_like(q, 9.0), ints([0])
+    assert rows * prefix * hk * d * 4 > 128 << 20
+    A.check(paged(cache, q, 1, trow, tpos, out, prefix, err=err))
+    check_rows(cache, q, 1, trow, tpos, out, dt)
+    assert err.item() == 0
+
+
+@pytest.mark.parametrize("qg,rows", [(1, 257), (3, 300), (2, 4000)])
+def test_paged_attention_many_groups(qg, rows):
+    """More groups than a CTA keeps, groups of several tokens, rows without keys and padding among them."""
+    h, hk, d, ps, dt = 8, 2, 64, 16, "bf16"
+    lens = [(1, 30, 0, 64, 129, 17, 300)[r % 7] for r in range(rows)]
+    lens = [n + qg - 1 if n else 0 for n in lens]
+    table, n_pages = tables(lens, ps)
+    cache, g = Paged(hk, d, ps, n_pages, dt, table), gen(rows)
+    fill_rows(cache, lens, g, dt)
+    trow = ints([r if r % 11 else -1 for r in range(rows) for _ in range(qg)])
+    tpos = ints([max(-1, n - qg + j) if n else -1 for n in lens for j in range(qg)])
+    q = rnd((rows * qg, h, d), g, dt)
+    out, err = torch.full_like(q, 9.0), ints([0])
+    A.check(paged(cache, q, qg, trow, tpos, out, err=err))
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    at = torch.arange(0, rows * qg, max(1, rows * qg // 400), device="cuda")
+    check_rows(cache, q[at], qg, trow[at], tpos[at], out[at], dt)
+    assert (out[trow < 0] == 9.0).all() and (out[(trow >= 0) & (tpos < 0)] == 0).all() and torch.isfinite(out).all()
+
+
+def test_shared_prefix_on_two_streams():
+    """Calls that read the prefix once, side by side on two streams, a workspace and queries each."""
+    x = Once(32, 8, 128, "f16", 2, 64, 2048, 600)
+    q0 = x.q
+    want = x.run()
+    x.check(want)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    wss = [torch.full((L.mlxcat_op_shared_prefix_attention_workspace(1200, 2, 32, 8, 128, 2048),), 0xff, dtype=torch.uint8, device="cuda")
+           for _ in streams]
+    qs = [q0, q0.flip(0).contiguous()]
+    rr, pp = [x.trow, x.trow.flip(0).contiguous()], [x.tpos, x.tpos.flip(0).contiguous()]
+    pp[1] = pp[1].view(-1, 2).flip(1).flatten().contiguous()      # within a group the positions rise again
+    qs[1] = qs[1].view(-1, 2, 32, 128).flip(1).flatten(0, 1).contiguous()
+    torch.cuda.synchronize()
+    for _ in range(15):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(torch.full_like(q0, 9.0))
+                A.check(paged(x.cache, qs[i], 2, rr[i], pp[i], outs[i][-1], x.prefix, ws=wss[i]))
+    torch.cuda.synchronize()
+    for o in outs[0]:
+        assert torch.equal(o, want)
+    for o in outs[1]:
+        x.q, x.trow, x.tpos = qs[1], rr[1], pp[1]
+        x.check(o)
+
+
+@pytest.mark.parametrize("h,hk,d,dt,at", [(8, 2, 128, "bf16", 0), (6, 2, 64, "f16", 8), (32, 8, 128, "f16", 24)])
+def test_packed_attention_on_slices_of_a_projection(h, hk, d, dt, at):
+    """q, k and v side by side in one buffer, the output on a 16-byte boundary."""
+    lens, g = [130, 1, 300], gen(at)
+    m, width = sum(lens), (h + 2 * hk) * d
+    x = rnd((m, width + 8), g, dt)
+    q, k, v = (x[:, a * d:(a + n) * d].unflatten(1, (n, d)) for a, n in ((0, h), (h, hk), (h + hk, hk)))
+    cu = ints([0, 130, 131, 431])
+    arena = torch.full((m * h * d + 64,), 9.0, dtype=DT[dt], device="cuda")
+    out = arena[at:at + m * h * d].view(m, h, d)
+    A.check(packed(q, k, v, cu, cu, 1, out, dt))
+    check_packed(q, k, v, cu, cu, 1, out, dt)
+    assert (arena[:at] == 9.0).all() and (arena[at + m * h * d:] == 9.0).all()
