@@ -482,8 +482,10 @@ MLXCAT_API int mlxcat_op_paged_attention(const mlxcat_paged_kv *kv, const void *
  * page_size pages for every row r of the batch): those pages are read once for
  * all tokens, on the tensor cores.  prefix_len 0 is mlxcat_op_paged_attention,
  * and so is a call whose rows would together read at most 128 MB of the prefix
- * (L2 serves that faster than a second pass and a join).  Where the prefix is
- * read once, a NaN or infinite V entry of it can reach tokens that see only a
+ * (L2 serves that about as fast as a second pass and a join).  It pays where
+ * the rows' own keys are shorter than the prefix: 64 rows over 2,048 shared keys
+ * 39 us against 69 with 256 keys of their own, but 217 against 176 with 4,096; a
+ * host that knows them to be long passes 0.  Where the prefix is read once, a NaN or infinite V entry of it can reach tokens that see only a
  * part of the prefix (tpos < prefix_len - 1). */
 MLXCAT_API size_t mlxcat_op_shared_prefix_attention_workspace(int32_t M, int32_t qg, int32_t n_heads,
                                                               int32_t n_kv_heads, int32_t head_dim,

@@ -16,6 +16,12 @@
 //                          reference m moves only when a row's maximum grows by
 //                          more than 8 (log2 units), so P <= 256 fits fp16.  P
 //                          goes back over the first half of its S buffer in TMEM.
+//                          It is rounded to the operands' 16 bits once, the sum of the
+//                          row is taken of the unrounded values in fp32.  A second part
+//                          would be a second product: the errors against 64 bits are
+//                          at most 1.4 times those of an fp32 P (fp16 2.3e-4 to 2.9e-4
+//                          against 2.0e-4, bf16 2.0e-3 to 2.4e-3 against 1.7e-3), and
+//                          an fp16 weight below 2^-25 of the reference vanishes.
 //   O_i += P_i V_j        A = P_i from TMEM, B = V_j read in place as an
 //                          MN-major operand
 // The two tiles take turns: while the tensor cores work for one, the other's
@@ -26,9 +32,9 @@
 // are zeroed in shared memory before the product, so what lies behind a
 // sequence (another prompt, an unwritten page, NaN) does not reach it.
 //
-// Measured on one B200 (32 query, 8 KV heads of 128): three prompts of 2,045 to
-// 6,144 tokens 540 us, 1.10 PFLOP/s of visible pairs (505 us, 1.18 in a short run
-// before the power limit lowers the clock); sixteen of 33 to 1,500 tokens 221 us.
+// Measured on B200s (32 query, 8 KV heads of 128): three prompts of 2,045 to
+// 6,144 tokens 557 us, 1.07 PFLOP/s of visible pairs (496 us, 1.20 in single launches
+// before the power limit lowers the clock); sixteen of 33 to 1,500 tokens 228 us.
 // A block of 64 keys takes a tile 1,650 cycles: its softmax 1,400 (the
 // exponentials of both tiles share 16 units, 1,024 cycles), the products of both
 // tiles about 1,500 (an MMA of 64 or 128 columns takes 58 to 65 cycles alike).  One
@@ -790,7 +796,11 @@ int prefix_splits(int M, int n_heads, int n_kv, int prefix_len, int sm_count) {
     // one wave of CTAs, two key blocks each at least; half a wave when a whole one
     // would have few blocks each: start and end of a CTA then count for more than
     // its blocks, and the rows' own keys are read on the other SMs meanwhile (64
-    // tokens over 8,192 shared keys: 46.7 us on all, 44.5 on a third, 41.3 on half)
+    // tokens over 8,192 shared keys and up to 512 own ones: 46.7 us on all, 44.5 on a
+    // third, 41.3 on half).  The host does not know the rows' own keys, and long ones
+    // behind a short prefix are better off without a pass: 64 rows of 32 / 8 heads over
+    // 2,048 shared keys took, read once against row by row, 39 and 69 us with 256 own
+    // keys, 77 and 93 with 1,024, 217 and 176 with 4,096, 810 and 688 with 16,384.
     int64_t sms = sm_count;
     if (blocks * items < FEW_BLOCKS * sms) sms /= 2;
     return (int)std::max<int64_t>(1, std::min<int64_t>(sms / items, (blocks + 1) / 2));

@@ -267,11 +267,12 @@ int mlxcat_op_shared_prefix_attention(const mlxcat_paged_kv *c, int32_t prefix_l
     PrefixPartials pre;
     const cudaStream_t st = (cudaStream_t)stream;
     // What the rows would read of the prefix one by one.  As long as that is about
-    // what L2 holds, reading it per row is the shorter way, since the pass over the
-    // shared keys and the join of its partials cost 12 us by themselves: 8 KV heads
-    // of 128, 32 rows, 256 keys (34 MB) 15 us per row against 22 us shared, 1,024
-    // keys (134 MB) 23 against 23, 64 rows and 1,024 keys (268 MB) 38 against 31,
-    // 4,096 keys (1.1 GB) 106 against 37.
+    // what L2 holds they do, since the pass over the shared keys and the join of its
+    // partials have a price of their own, which grows with the rows' own keys (they get
+    // half the SMs).  8 KV heads of 128, row by row against once, 64 and 1,024 own keys:
+    // 32 rows, 256 shared keys (34 MB) 14 and 31 us against 17 and 40; 32 rows, 1,024
+    // keys (134 MB) 24 against 17 with 64 own keys; 64 rows, 1,024 keys (268 MB) 38 and
+    // 63 against 21 and 62; 64 rows, 4,096 keys (1.1 GB) 111 against 27.
     const int64_t apart = (int64_t)((M + pq.qg - 1) / pq.qg) * prefix_len * kv.n_kv * kv.D * 4;
     if (apart <= ((int64_t)128 << 20)) prefix_len = 0;
     if (prefix_len) {

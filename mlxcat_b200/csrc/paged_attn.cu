@@ -25,10 +25,11 @@
 //
 // Two CTAs of four warps an SM keep 128 KB of loads in flight; with two or one
 // warp a CTA (four or six CTAs) 64 rows of up to 16k keys took 395 and 308 us
-// against 298.  Measured on one B200: those 64 rows (64 query heads, 8 KV heads of
-// 128, bf16) 298 us, 6.3 TB/s, 0.97 of the copy rate; 32 x 5 verify tokens over
-// 4.2k keys 103 us, 5.3 TB/s.  What is left there is the start (the lengths, the
-// page ids and the first keys are one chain of loads, 3 us) and the join.
+// where two of four took 298.  Measured on B200s: those 64 rows (64 query heads, 8
+// KV heads of 128, bf16) 304 us, 6.2 TB/s, 0.95 of the copy rate; 32 x 5 verify
+// tokens over 4.2k keys 106 to 110 us, 5.0 to 5.2 TB/s.  What is left there is the
+// start (the lengths, the page ids and the first keys are one chain of loads, 3 us)
+// and the join.
 #include <algorithm>
 
 #include "common.cuh"
@@ -161,7 +162,10 @@ struct PagedShape {
     static constexpr int SMEM = BODY + TAIL;
 };
 constexpr int NOBODY = 0x7fffffff;   // key limit of query rows that are padding or behind the group
-constexpr int MAX_GROUPS = 256;   // groups whose (row, last key) a CTA keeps
+// Groups whose (row, last key) a CTA keeps; beyond, it reads them again from the
+// descriptors.  Rows of 1,024 keys (32 / 8 heads of 128): 256 rows 178 us, 257 180,
+// 512 340, 2,048 1,340; groups of 5 tokens: 256 rows 224 us, 257 223, 512 398.
+constexpr int MAX_GROUPS = 256;
 
 // 8 features of a query row on their way through partials.
 struct Joined {
@@ -815,9 +819,15 @@ cudaError_t run(const PagedKV &kv, const PagedQuery &q, int key_begin, const Pre
     const int64_t cap = std::max(0, paged_capacity(kv) - key_begin);
     const int64_t units = (int64_t)s.items * ((cap + UNIT - 1) / UNIT + LEAD);
     // Beside a prefix pass that leaves SMs free, this kernel takes those and no more:
-    // CTAs that had to wait for the pass would be the last.
+    // CTAs that had to wait for the pass would be the last.  That is for own keys that
+    // are short beside the prefix, as prefix_splits says with both sides' times; with
+    // long ones (which only the device knows) the SMs of the pass are missed.
     const int free_sms = pre.splits && pre.ctas <= sm_count - sm_count / 4 ? sm_count - pre.ctas : sm_count;
-    // few units: one cluster that joins its own pieces, no second kernel
+    // few units: one cluster that joins its own pieces, no second kernel (one row of
+    // 300 keys, 8 / 2 heads of 64, 7.95 -> 7.2 us).  The host knows no lengths, so the
+    // table's width decides: up to 1,856 keys for one row with two KV heads, 320 for
+    // four rows.  A wider table takes the two kernels; back to back on the same inputs
+    // that is one row 7.2 us either way, four rows 8.1 us here and 7.5 there.
     const bool cluster = units <= ONE_CLUSTER * CLUSTER_UNITS;
     const int grid = (int)std::min<int64_t>(cluster ? ONE_CLUSTER : (int64_t)free_sms * CTAS_PER_SM, units);
     cudaError_t e;
