@@ -224,17 +224,17 @@ __device__ __forceinline__ Work work_of(const Args &a, int id) {
         int lo = 0, n = a.n_seq;
         while (n > 32) {
             const int step = (n + 31) / 32, at = lo + lane * step;
-            const bool in = lane * step < n && __ldg(a.cu_q + at) / (2 * a.TQ) + at <= tile;
+            const bool in = lane * step < n && load_id(a.cu_q + at) / (2 * a.TQ) + at <= tile;
             const int k = max(__popc(__ballot_sync(0xffffffffu, in)) - 1, 0);
             lo += k * step;
             n = min(step, n - k * step);
         }
         int c[4] = {0, 0, 0, 0};
         if (lane < n) {
-            c[0] = __ldg(a.cu_q + lo + lane);
-            c[1] = __ldg(a.cu_q + lo + lane + 1);
-            c[2] = __ldg(a.cu_k + lo + lane);
-            c[3] = __ldg(a.cu_k + lo + lane + 1);
+            c[0] = load_id(a.cu_q + lo + lane);
+            c[1] = load_id(a.cu_q + lo + lane + 1);
+            c[2] = load_id(a.cu_k + lo + lane);
+            c[3] = load_id(a.cu_k + lo + lane + 1);
         }
         const int k = max(__popc(__ballot_sync(0xffffffffu, lane < n && c[0] / (2 * a.TQ) + lo + lane <= tile)) - 1, 0);
 #pragma unroll
@@ -356,7 +356,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             // any row's table will do: the first token's that is no padding
             int row = -1;
             for (int m0 = 0; m0 < a.M && row < 0; m0 += 32) {
-                const int r = m0 + lane < a.M ? __ldg(a.trow + m0 + lane) : -1;
+                const int r = m0 + lane < a.M ? load_id(a.trow + m0 + lane) : -1;
                 const unsigned ok = __ballot_sync(0xffffffffu, r >= 0 && r < a.kv.rows);
                 if (ok) row = __shfl_sync(0xffffffffu, r, __ffs(ok) - 1);
             }
@@ -420,7 +420,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                         const int b = lane / S::HALVES, x = lane % S::HALVES;
                         if (a.prefix) {
                             const int key = key0 + b * bt;
-                            int page = table ? __ldg(table + (key >> a.kv.page_shift)) : -1;
+                            int page = table ? load_id(table + (key >> a.kv.page_shift)) : -1;
                             if (page < 0 || page >= a.kv.n_pages) {   // reads as zeros (a box outside the tensor)
                                 if (table && a.err) atomicExch(a.err, PE_PAGE);
                                 page = a.kv.n_pages;
@@ -587,7 +587,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             if (valid) {
                 if (!a.prefix) lim = a.causal ? min(w.first_lim + tk, w.kend - 1) : w.kend - 1;
                 else {
-                    const int row = __ldg(a.trow + w.tok0 + tk), pos = __ldg(a.tpos + w.tok0 + tk);
+                    const int row = load_id(a.trow + w.tok0 + tk), pos = load_id(a.tpos + w.tok0 + tk);
                     pad = row < 0;
                     if (row < a.kv.rows) lim = min(pos, w.kend - 1);   // a row outside the table sees nothing
                 }

@@ -33,6 +33,12 @@ __host__ __device__ inline int paged_capacity(const PagedKV &kv) {
     return c > 0x7fff0000 ? 0x7fff0000 : (int)c;
 }
 
+// Everything that these kernels read may be written by the kernel before, and they
+// are launched early (programmatic serialisation): plain loads, since the read-only
+// path (ld.global.nc) is for memory that nobody writes while the kernel lives, and
+// neither griddepcontrol.wait nor an acquire orders it.
+__device__ __forceinline__ int load_id(const int32_t *p) { return *p; }
+
 struct RopeAppendArgs {
     const void *q, *k, *v;
     int64_t q_stride, k_stride, v_stride;   // elements between tokens

@@ -101,10 +101,6 @@ __device__ __forceinline__ void cpa16(uint32_t s, const void *g, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(g), "r"(bytes) : "memory");
 }
 
-// Tokens' rows and positions and page ids: plain loads, since an acquire orders
-// them and does not order loads by the read-only path.
-__device__ __forceinline__ int load_id(const int32_t *p) { return *p; }
-
 // What a group of tokens sees: its row and one past its last key.
 struct Group {
     int row, kend;

@@ -86,7 +86,10 @@ struct Vec8 {
     uint4 w[W];
     __device__ __forceinline__ void load(const TI *p) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        for (int i = 0; i < W; ++i)   // volatile: behind griddep_wait; nothing the kernel writes is read here
+            asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+                         : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                         : "l"(reinterpret_cast<const uint4 *>(p) + i));
     }
     __device__ __forceinline__ void get(uint64_t *x) const {
 #pragma unroll
@@ -121,7 +124,7 @@ rope_append_kernel(const PagedKV kv, const __grid_constant__ mlxcat_rope rope, c
     if (norms) {
         for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
             const float *w = i < D ? a.q_norm : a.k_norm;
-            if (w) nw[i / D][i % D] = __ldg(w + i % D);
+            if (w) nw[i / D][i % D] = w[i % D];
         }
         __syncthreads();
     }
@@ -147,14 +150,14 @@ rope_append_kernel(const PagedKV kv, const __grid_constant__ mlxcat_rope rope, c
     Vec8<TI> cur[RA_BATCH][2], nxt[RA_BATCH][2];
     int m = u / chunks, h0 = (u - m * chunks) * per * HPI, mn = m, hn = h0;   // of this unit and the next
     fetch(m, h0, 0, cur);
-    int row = __ldg(a.trow + m), pos = __ldg(a.tpos + m);
+    int row = load_id(a.trow + m), pos = load_id(a.tpos + m);
     for (; u < units; u += nwarps, m = mn, h0 = hn) {
         // the token's slot; one outside the table or the cache is not written
         int bad = 0, page = 0;
         if (row >= kv.rows) bad = PE_ROW;
         else if (pos < 0 || pos >= paged_capacity(kv)) bad = PE_POS;
         else if (row >= 0) {
-            page = __ldg(kv.table + (size_t)row * kv.max_pages + (pos >> kv.page_shift));
+            page = load_id(kv.table + (size_t)row * kv.max_pages + (pos >> kv.page_shift));
             if (page < 0 || page >= kv.n_pages) bad = PE_PAGE;
         }
         const int64_t at = bad ? -1 : (int64_t)page * kv.page_stride + (int64_t)(pos & ((1 << kv.page_shift) - 1)) * kv.token_stride;
@@ -182,8 +185,8 @@ rope_append_kernel(const PagedKV kv, const __grid_constant__ mlxcat_rope rope, c
         if (u + nwarps < units) {
             mn = (u + nwarps) / chunks;
             hn = (u + nwarps - mn * chunks) * per * HPI;
-            row = __ldg(a.trow + mn);
-            pos = __ldg(a.tpos + mn);
+            row = load_id(a.trow + mn);
+            pos = load_id(a.tpos + mn);
         }
 #pragma unroll 1
         for (int round = 0; round < per; round += RA_BATCH) {

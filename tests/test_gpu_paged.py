@@ -1066,3 +1066,44 @@ def test_packed_attention_on_slices_of_a_projection(h, hk, d, dt, at):
     A.check(packed(q, k, v, cu, cu, 1, out, dt))
     check_packed(q, k, v, cu, cu, 1, out, dt)
     assert (arena[:at] == 9.0).all() and (arena[at + m * h * d:] == 9.0).all()
+
+
+@pytest.mark.parametrize("m", [8, 160])
+def test_projection_append_attention_launched_early(m):
+    """Each kernel of the chain starts before the one in front has ended, on memory that has just been read with
+    other contents: what is read is what that one wrote."""
+    h, hk, d, ps, qg, dt = 8, 2, 128, 64, 4, "f16"
+    rows, n, kk, g = m // qg, (h + 2 * hk) * d, 512, gen(m)
+    wq = torch.randint(-2 ** 31, 2 ** 31 - 1, (n, kk // 8), dtype=torch.int32, device="cuda", generator=g)
+    sc, bi = ((torch.rand((n, kk // 64), device="cuda", generator=g) * 0.01 + b).half() for b in (0.005, -0.1))
+    xs = [rnd((m, kk), g, dt) for _ in range(3)]
+    lens = [70 + 3 * r for r in range(rows)]
+    table, n_pages = tables([x + qg for x in lens], ps)
+    cache = Paged(hk, d, ps, n_pages, dt, table)
+    fill_rows(cache, [x + qg for x in lens], g, dt)
+    trow = ints([r for r in range(rows) for _ in range(qg)])
+    ends = [ints([x + j - s for x in lens for j in range(qg)]) for s in (0, 40, 11)]
+    tpos, x = ends[0].clone(), xs[0].clone()
+    y = torch.zeros((m, n), device="cuda")
+    q_out, out = torch.zeros((m, h, d), dtype=torch.float16, device="cuda"), torch.zeros((m, h, d), dtype=torch.float16, device="cuda")
+    size = L.mlxcat_op_q4_linear_workspace(n, kk, m)
+    lw, ws = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty(
+        L.mlxcat_op_paged_attention_workspace(m, qg, h, hk, d), dtype=torch.uint8, device="cuda")
+    seen = set()
+    for i in range(30):
+        x.copy_(xs[i % 3])
+        tpos.copy_(ends[i % 3 if i % 2 else 0])
+        A.check(L.mlxcat_op_q4_linear(ptr(wq), ptr(sc), ptr(bi), n, kk, ptr(x), m, ptr(y), ptr(lw), size, stream()))
+        A.check(append(cache, None, y[:, :h * d], y[:, h * d:(h + hk) * d], y[:, (h + hk) * d:], "f32", trow, tpos, q_out))
+        A.check(paged(cache, q_out, qg, trow, tpos, out, ws=ws))
+        torch.cuda.synchronize()
+        half = y.half()
+        assert torch.isfinite(half).all() and half.float().std() > 0.05
+        assert torch.equal(q_out.view(m, -1), half[:, :h * d])
+        page, off = table[trow.long(), (tpos // ps).long()].long(), (tpos % ps).long()
+        assert torch.equal(cache.k[page, :, off].reshape(m, -1), half[:, h * d:(h + hk) * d])
+        assert torch.equal(cache.v[page, :, off].reshape(m, -1), half[:, (h + hk) * d:])
+        at = torch.arange(0, m, 7, device="cuda")
+        check_rows(cache, q_out[at], qg, trow[at], tpos[at], out[at], dt)
+        seen.add(round(y.double().sum().item(), 3))
+    assert len(seen) == 3
