@@ -468,8 +468,9 @@ MLXCAT_API int mlxcat_op_rope_append(const mlxcat_paged_kv *kv, const mlxcat_rop
  * A token that sees no key (tpos < 0) gets zeros, a padding token's output is
  * left as it was.  A row outside the table sets *err (device int, may be NULL)
  * and its tokens get zeros; a position outside sets it and is cut to the table; a
- * page id outside the cache sets it and reads as zeros.  Keys past a group's last position are not read; a NaN or
- * infinite V entry reaches every token of a group that may see it. */
+ * page id outside the cache sets it and reads as zeros.  Keys past a group's last
+ * position are not read; a NaN or infinite V entry reaches every token of a group
+ * that may see it. */
 MLXCAT_API size_t mlxcat_op_paged_attention_workspace(int32_t M, int32_t qg, int32_t n_heads, int32_t n_kv_heads,
                                                       int32_t head_dim);
 MLXCAT_API int mlxcat_op_paged_attention(const mlxcat_paged_kv *kv, const void *q, int32_t M, int32_t qg,
@@ -485,8 +486,9 @@ MLXCAT_API int mlxcat_op_paged_attention(const mlxcat_paged_kv *kv, const void *
  * (L2 serves that about as fast as a second pass and a join).  It pays where
  * the rows' own keys are shorter than the prefix: 64 rows over 2,048 shared keys
  * 39 us against 69 with 256 keys of their own, but 217 against 176 with 4,096; a
- * host that knows them to be long passes 0.  Where the prefix is read once, a NaN or infinite V entry of it can reach tokens that see only a
- * part of the prefix (tpos < prefix_len - 1). */
+ * host that knows them to be long passes 0.  Where the prefix is read once, a
+ * NaN or infinite V entry of it can reach tokens that see only a part of the
+ * prefix (tpos < prefix_len - 1). */
 MLXCAT_API size_t mlxcat_op_shared_prefix_attention_workspace(int32_t M, int32_t qg, int32_t n_heads,
                                                               int32_t n_kv_heads, int32_t head_dim,
                                                               int32_t prefix_len);

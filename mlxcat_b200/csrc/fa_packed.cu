@@ -33,8 +33,9 @@
 // sequence (another prompt, an unwritten page, NaN) does not reach it.
 //
 // Measured on B200s (32 query, 8 KV heads of 128): three prompts of 2,045 to
-// 6,144 tokens 557 us, 1.07 PFLOP/s of visible pairs (496 us, 1.20 in single launches
-// before the power limit lowers the clock); sixteen of 33 to 1,500 tokens 228 us.
+// 6,144 tokens 551 to 558 us, 1.07 PFLOP/s of visible pairs (496 us, 1.20 in single
+// launches before the power limit lowers the clock); sixteen of 33 to 1,500 tokens
+// 226 to 229 us.
 // A block of 64 keys takes a tile 1,650 cycles: its softmax 1,400 (the
 // exponentials of both tiles share 16 units, 1,024 cycles), the products of both
 // tiles about 1,500 (an MMA of 64 or 128 columns takes 58 to 65 cycles alike).  One

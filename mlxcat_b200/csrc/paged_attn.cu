@@ -26,7 +26,7 @@
 // Two CTAs of four warps an SM keep 128 KB of loads in flight; with two or one
 // warp a CTA (four or six CTAs) 64 rows of up to 16k keys took 395 and 308 us
 // where two of four took 298.  Measured on B200s: those 64 rows (64 query heads, 8
-// KV heads of 128, bf16) 304 us, 6.2 TB/s, 0.95 of the copy rate; 32 x 5 verify
+// KV heads of 128, bf16) 303 to 307 us, 6.2 TB/s, 0.95 of the copy rate; 32 x 5 verify
 // tokens over 4.2k keys 106 to 110 us, 5.0 to 5.2 TB/s.  What is left there is the
 // start (the lengths, the page ids and the first keys are one chain of loads, 3 us)
 // and the join.

@@ -20,7 +20,8 @@
 // 16,396 tokens of 32 + 2 * 8 heads, bf16, normalised, interleaved), groups of four
 // tokens a CTA still on the barrier (89 us), a warp a token with every lane
 // choosing between q, k and v for itself 80 us; now 73 us, 5.5 TB/s, 0.84 of the
-// copy rate, and the instruction rate bounds it (70 % of issue slots).  160 tokens of an fp32 projection: 4.6 us, launch-bound.
+// copy rate, and the instruction rate bounds it (70 % of issue slots).  160 tokens
+// of an fp32 projection: 4.5 to 4.9 us, launch-bound.
 #include <algorithm>
 
 #include "common.cuh"
